@@ -1,0 +1,20 @@
+// What a launch of AdamW takes (mirrored by distributed_tensorflow_amd/optim/adamw.py).
+#pragma once
+#include <stdint.h>
+
+struct AdamWLaunch {
+  const int64_t* shape;   // [ntensors][2]: elements, place in the arenas
+  const void* chunks;     // [nchunks] {tensor, chunk of 2048 elements in it}
+  void* live;             // [ntensors] written by the first kernel for the second
+  int* step;              // [ntensors]
+  void* m;                // arenas: float, or e4m3 ...
+  void* v;                // ... (r = sqrt(v) in 8 bits)
+  float* m_scale;         // [arena / 256], 8 bits only
+  float* r_scale;
+  double lr, beta1, beta2;
+  float b1, ob1, b2, ob2; // b, 1 - b, each rounded once
+  float eps, decay;       // decay = 1 - lr * weight_decay
+  float grad_scale;
+  uint32_t seed;
+  int ntensors, nchunks, bits;
+};
