@@ -9,6 +9,7 @@ composed with ``nn.Module`` and trained with any ``torch.optim`` optimizer (or `
 * ``conv_bn_relu(x, w, gamma, beta, ...)``  — any Inception geometry, training-mode BatchNorm (statistics in the
                                               conv epilogue) + ReLU, NHWC bf16 in/out
 * ``max_pool3x3(x, stride)`` / ``avg_pool3x3_same(x)``
+* ``rms_norm(x, weight, residual)``         — norm over the last dimension with the residual's addition, any rows (fp32 or bf16)
 
 Activations are NHWC bf16, parameters fp32 (converted to bf16 while staged into LDS), gradients of parameters fp32,
 gradients of activations bf16 — exactly the conventions of the static engines, whose tests these wrappers share.
@@ -19,6 +20,7 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from .. import native
 from . import hip_ops
@@ -235,7 +237,44 @@ def avg_pool3x3_same(x: torch.Tensor) -> torch.Tensor:
     return _AvgPool3x3Same.apply(x)
 
 
+class _RMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps: float):
+        y, h, rstd = hip_ops.rms_norm_forward(x, weight, residual, eps)
+        ctx.save_for_backward(x, rstd, weight, residual)
+        ctx.set_materialize_grads(False)
+        return y if residual is None else (y, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        x, rstd, weight, residual = ctx.saved_tensors
+        need_x, need_w, need_r, _ = ctx.needs_input_grad
+        if dy is None:  # only h went into the loss
+            return dh if need_x else None, torch.zeros_like(weight) if need_w else None, dh if need_r else None, None
+        dx, dw = hip_ops.rms_norm_backward(dy, x, rstd, weight, residual, dh, need_dw=need_w)
+        return dx if need_x else None, dw, dx if need_r else None, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """``h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension; ``y``, or ``(y, h)`` with a residual.
+    ``x`` and ``residual`` fp32 or bf16 of one shape and type, ``weight`` fp32; differentiable once in all three."""
+    return _RMSNorm.apply(x, weight, residual, eps)
+
+
 # ------------------------------------------------------------------------------------------------ layers
+class RMSNorm(nn.Module):
+    """``rms_norm`` with a learned weight: ``forward(x)`` -> y, ``forward(x, residual)`` -> ``(y, x + residual)``."""
+
+    def __init__(self, dim: int, eps: float = 1e-6):
+        super().__init__()
+        self.weight = nn.Parameter(torch.ones(dim))
+        self.eps = eps
+
+    def forward(self, x, residual=None):
+        return rms_norm(x, self.weight, residual, self.eps)
+
+
 class Linear(nn.Module):
     """Dense layer with TensorFlow-layout ``[in, out]`` fp32 weights on the MFMA GEMM."""
 
