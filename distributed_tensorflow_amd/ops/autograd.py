@@ -9,6 +9,7 @@ composed with ``nn.Module`` and trained with any ``torch.optim`` optimizer (or `
 * ``conv_bn_relu(x, w, gamma, beta, ...)``  — any Inception geometry, training-mode BatchNorm (statistics in the
                                               conv epilogue) + ReLU, NHWC bf16 in/out
 * ``max_pool3x3(x, stride)`` / ``avg_pool3x3_same(x)``
+* ``LinearW4.from_linear(layer)``           — a trained dense layer with 4-bit weights, for inference
 * ``rms_norm(x, weight, residual)``         — norm over the last dimension with the residual's addition, any rows (fp32 or bf16)
 
 Activations are NHWC bf16, parameters fp32 (converted to bf16 while staged into LDS), gradients of parameters fp32,
@@ -288,6 +289,28 @@ class Linear(nn.Module):
 
     def forward(self, x):
         return linear(x, self.weight, self.bias, self.relu)
+
+
+class LinearW4(nn.Module):
+    """A trained ``Linear`` with 4-bit weights, for inference (``hip_ops.linear_w4``): ``LinearW4.from_linear(layer, group=64)``."""
+
+    def __init__(self, in_features: int, out_features: int, relu: bool = False, group: int = 64):
+        super().__init__()
+        wq, scales = hip_ops.quantize_w4(torch.zeros(in_features, out_features), group)
+        self.register_buffer("wq", wq)
+        self.register_buffer("scales", scales)
+        self.register_buffer("bias", torch.zeros(out_features))
+        self.in_features, self.out_features, self.relu = in_features, out_features, relu
+
+    @classmethod
+    def from_linear(cls, layer: Linear, group: int = 64) -> "LinearW4":
+        q = cls(*layer.weight.shape, relu=layer.relu, group=group)
+        q.wq, q.scales = hip_ops.quantize_w4(layer.weight.detach(), group)
+        q.bias = layer.bias.detach().clone()
+        return q
+
+    def forward(self, x, x_scale=None):
+        return hip_ops.linear_w4(x, self.wq, self.scales, self.out_features, self.bias, self.relu, x_scale)
 
 
 class ConvReluPool(nn.Module):

@@ -441,3 +441,110 @@ def rms_norm_backward(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, wei
     a.rows, a.dim, a.bf16, a.blocks = rows, dim, x.dtype == torch.bfloat16, blocks
     _launch(x, "rms_norm_bwd", lib.dtf_rms_norm_bwd, C.byref(a))
     return dx, dw
+
+
+# ----------------------------------------------------------------------------- dense layers with 4-bit weights (csrc/hip/linear_w4.hip)
+class LinearW4Args(C.Structure):  # csrc/hip/linear_w4.hip
+    _fields_ = [("x", C.c_void_p), ("wq", C.c_void_p), ("scales", C.c_void_p), ("bias", C.c_void_p), ("x_scale", C.c_void_p),
+                ("y", C.c_void_p), ("M", C.c_long), ("ldx", C.c_long), ("N", C.c_int), ("K", C.c_int), ("group", C.c_int),
+                ("xtype", C.c_int), ("relu", C.c_int), ("out_bf16", C.c_int)]
+
+
+native.register_hip_sig("dtf_sizeof_linear_w4_args", C.c_int, [])
+native.register_hip_sig("dtf_linear_w4", C.c_int, [C.POINTER(LinearW4Args), C.c_void_p])
+
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+_X_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
+W4_MAX_ROWS = 65535 * 5
+
+
+def quantize_w4(w: torch.Tensor, group: int = 64) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp32 or bf16 weights ``w[K,N]`` -> ``(wq, scales)`` for ``linear_w4``, on any device; ``group``: 32, 64 or 128 successive k share a scale.
+
+    A weight is ``e2m1(code) * scale``: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives, to nearest (ties to the even code); the scale is
+    the group's largest magnitude / 6 in bf16.  ``wq`` uint8 ``[ceil(N/16), ceil(K/128), 64, 16]``: entry ``16 * (k % 32 // 8) + n % 16`` holds the codes
+    of output n, byte ``4 * (k % 128 // 32) + k % 8 // 2``, low nibble first; ``scales`` bf16 ``[ceil(N/16), ceil(K/128) * 128/group, 16]``.  What is behind
+    the last row or column is zero."""
+    if group not in (32, 64, 128):
+        raise ValueError("group is 32, 64 or 128 (got %r)" % (group,))
+    if w.dim() != 2 or w.dtype not in (torch.float32, torch.bfloat16) or w.numel() == 0:
+        raise ValueError("w must be float32 or bfloat16 [K, N] weights (got %s %s)" % (w.dtype, tuple(w.shape)))
+    if not bool(torch.isfinite(w).all()):
+        raise ValueError("weights that are not finite have no 4-bit form")
+    K, N = w.shape
+    kt, nt = -(-K // 128), -(-N // 16)
+    full = torch.zeros(kt * 128, nt * 16, dtype=torch.float32, device=w.device)
+    full[:K, :N] = w
+    g = full.view(-1, group, nt * 16)
+    scale = (g.abs().amax(1) / 6).to(torch.bfloat16)
+    # (the smallest normal float: a bf16 scale that rounds to zero, or is denormal, holds zeros)
+    scale = torch.where(scale.float() < 2.0 ** -126, 0.0, scale.float())
+    v = (g / torch.where(scale > 0, scale, 1.0)[:, None]) * (scale > 0)[:, None]
+    a = v.abs()
+    code = ((a > 0.25).to(torch.uint8) + (a >= 0.75).to(torch.uint8) + (a > 1.25).to(torch.uint8) + (a >= 1.75).to(torch.uint8)
+            + (a > 2.5).to(torch.uint8) + (a >= 3.5).to(torch.uint8) + (a > 5).to(torch.uint8))
+    code |= (v < 0).to(torch.uint8) << 3
+    c = code.view(kt, 4, 4, 4, 2, nt, 16)  # k tile, instruction, lane group, byte, nibble; n tile, n
+    c = c.permute(5, 0, 2, 6, 1, 3, 4).reshape(nt, kt, 64, 16, 2)
+    s = scale.to(torch.bfloat16).view(-1, nt, 16).permute(1, 0, 2).contiguous()
+    return (c[..., 0] | (c[..., 1] << 4)).contiguous(), s
+
+
+def _w4_group(wq: torch.Tensor, scales: torch.Tensor) -> int:
+    """The group size of a pair from ``quantize_w4``, checked."""
+    ok = (wq.dtype == torch.uint8 and wq.dim() == 4 and wq.shape[2:] == (64, 16) and wq.is_contiguous() and wq.numel() > 0
+          and scales.dtype == torch.bfloat16 and scales.dim() == 3 and scales.is_contiguous() and scales.shape[0] == wq.shape[0]
+          and scales.shape[2] == 16 and scales.shape[1] in (wq.shape[1], 2 * wq.shape[1], 4 * wq.shape[1]) and scales.device == wq.device)
+    if not ok:
+        raise ValueError("not a pair from quantize_w4: %s %s, %s %s" % (wq.dtype, tuple(wq.shape), scales.dtype, tuple(scales.shape)))
+    return wq.shape[1] * 128 // scales.shape[1]
+
+
+def dequantize_w4(wq: torch.Tensor, scales: torch.Tensor, in_features: int, out_features: int) -> torch.Tensor:
+    """The fp32 weights ``[in_features, out_features]`` that ``quantize_w4``'s result stands for."""
+    group = _w4_group(wq, scales)
+    nt, kt = wq.shape[:2]
+    if not (0 < in_features <= kt * 128 and 0 < out_features <= nt * 16):
+        raise ValueError("%d x %d features in %d x %d tiles" % (in_features, out_features, kt, nt))
+    c = torch.stack((wq & 15, wq >> 4), -1).view(nt, kt, 4, 16, 4, 4, 2).permute(1, 4, 2, 5, 6, 0, 3).reshape(kt * 128, nt * 16)
+    table = torch.tensor(_E2M1 + tuple(-v for v in _E2M1), device=wq.device)
+    s = scales.float().permute(1, 0, 2).reshape(scales.shape[1], nt * 16).repeat_interleave(group, 0)
+    return (table[c.int()] * s)[:in_features, :out_features].contiguous()
+
+
+def linear_w4(x: torch.Tensor, wq: torch.Tensor, scales: torch.Tensor, out_features: int, bias: Optional[torch.Tensor] = None,
+              relu: bool = False, x_scale: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """``relu?((x * x_scale) @ W + bias)`` with the weights of ``quantize_w4``, for inference: made for a single row and a few dozen.
+
+    ``x[..., K]`` fp32 (not rounded), bf16, or e4m3 with ``x_scale`` (fp32, one a row; as ``rms_norm_e4m3`` gives them; optional for
+    the other types); any stride between rows.  ``bias`` fp32 ``[out_features]``; the result fp32 or bf16 ``[..., out_features]``.  Sums are fp32.
+    More than 64 rows (fp32: 10) read the weights again for each further 64."""
+    group = _w4_group(wq, scales)
+    if not x.is_cuda or x.dtype not in _X_TYPES or x.dim() < 1 or x.device != wq.device:
+        raise ValueError("x must be a CUDA tensor of float32, bfloat16 or float8_e4m3fn on the weights' device (got %s on %s)" % (x.dtype, x.device))
+    K, N = x.shape[-1], int(out_features)
+    if K < 1 or -(-K // 128) != wq.shape[1] or N < 1 or -(-N // 16) != wq.shape[0]:
+        raise ValueError("x %s and %d outputs do not fit weights of %d x %d tiles of 128 x 16" % (tuple(x.shape), N, wq.shape[1], wq.shape[0]))
+    if out_dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("out_dtype is float32 or bfloat16 (got %s)" % (out_dtype,))
+    if x_scale is None and x.dtype == torch.float8_e4m3fn:
+        raise ValueError("e4m3 rows need their x_scale")
+    for t, name, n in ((bias, "bias", N), (x_scale, "x_scale", x.numel() // K)):
+        if t is not None:
+            _chk(t, torch.float32, name)
+            if t.numel() != n or t.device != x.device:
+                raise ValueError("%s has %d elements on %s, not %d on %s" % (name, t.numel(), t.device, n, x.device))
+    y = torch.empty(x.shape[:-1] + (N,), dtype=out_dtype, device=x.device)
+    if not x.numel():
+        return y
+    x2 = x if x.dim() == 2 else x.reshape(-1, K)
+    if K > 1 and x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    if x2.shape[0] > W4_MAX_ROWS:
+        raise ValueError("at most %d rows (got %d)" % (W4_MAX_ROWS, x2.shape[0]))
+    a = LinearW4Args()
+    a.x, a.wq, a.scales, a.bias, a.x_scale, a.y = x2.data_ptr(), wq.data_ptr(), scales.data_ptr(), native.ptr(bias), native.ptr(x_scale), y.data_ptr()
+    a.M, a.ldx, a.N, a.K, a.group, a.xtype = x2.shape[0], x2.stride(0), N, K, group, _X_TYPES[x.dtype]
+    a.relu, a.out_bf16 = relu, out_dtype == torch.bfloat16
+    _launch(x, "linear_w4", native.hip().dtf_linear_w4, C.byref(a))
+    return y

@@ -1,0 +1,79 @@
+"""The 4-bit weights' format (on the CPU), and refusals of the product that need no GPU."""
+import ctypes
+
+import pytest
+import torch
+
+VALUES = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+
+
+@pytest.mark.parametrize("K,N", [(1, 1), (128, 16), (129, 17), (300, 40), (32, 100)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantized_weights_are_the_nearest_values(K, N, group, dtype):
+    from distributed_tensorflow_amd.ops import hip_ops
+    w = torch.randn(K, N, generator=torch.Generator().manual_seed(K + N)).to(dtype)
+    wq, scales = hip_ops.quantize_w4(w, group)
+    assert wq.shape == (-(-N // 16), -(-K // 128), 64, 16) and scales.shape == (-(-N // 16), -(-K // 128) * 128 // group, 16)
+    back = hip_ops.dequantize_w4(wq, scales, K, N)
+    table = torch.tensor(VALUES + [-v for v in VALUES], dtype=torch.float64)
+    for k in range(0, K, max(1, K // 40)):  # straight from the documented layout
+        for n in range(N):
+            byte = int(wq[n // 16, k // 128, 16 * (k % 32 // 8) + n % 16, 4 * (k % 128 // 32) + k % 8 // 2])
+            s = float(scales[n // 16, k // group, n % 16])
+            top = float(w[k // group * group:(k // group + 1) * group, n].abs().max())
+            assert abs(s - top / 6) <= top / 6 * 2.0 ** -8
+            value = float(table[byte >> 4 if k % 2 else byte & 15]) * s
+            assert value == float(back[k, n])
+            # no other value of the scaled table is nearer, up to the rounding of w / s
+            assert abs(float(w[k, n]) - value) <= float((table * s - float(w[k, n])).abs().min()) + 1e-6 * top
+    full = hip_ops.dequantize_w4(wq, scales, -(-K // 128) * 128, -(-N // 16) * 16)
+    assert not full[K:].any() and not full[:, N:].any()
+
+
+def test_ties_go_to_the_even_code_and_zeros_stay():
+    from distributed_tensorflow_amd.ops import hip_ops
+    w = torch.zeros(32, 2)
+    ties = [0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0]
+    w[:7, 0], w[7, 0], w[8:15, 0] = torch.tensor(ties), 6.0, -torch.tensor(ties)
+    wq, scales = hip_ops.quantize_w4(w, 32)
+    back = hip_ops.dequantize_w4(wq, scales, 32, 2)
+    assert back[:7, 0].tolist() == [0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0] and back[8:15, 0].tolist() == [-0.0, -1.0, -1.0, -2.0, -2.0, -4.0, -4.0]
+    assert not back[:, 1].any() and float(scales[0, 0, 1]) == 0
+    tiny = hip_ops.dequantize_w4(*hip_ops.quantize_w4(torch.full((32, 1), 1e-45), 32), 32, 1)
+    assert not tiny.any()
+
+
+def test_refusals():
+    from distributed_tensorflow_amd.ops import autograd, hip_ops
+    w = torch.randn(64, 32)
+    for bad in (lambda: hip_ops.quantize_w4(w, 16), lambda: hip_ops.quantize_w4(w.double()), lambda: hip_ops.quantize_w4(w[0]),
+                lambda: hip_ops.quantize_w4(w[:0]), lambda: hip_ops.quantize_w4(torch.full((4, 4), float("inf")))):
+        with pytest.raises(ValueError):
+            bad()
+    wq, scales = hip_ops.quantize_w4(w)
+    for bad in (lambda: hip_ops.dequantize_w4(wq, scales, 64, 33), lambda: hip_ops.dequantize_w4(wq, scales, 129, 32),
+                lambda: hip_ops.dequantize_w4(wq, scales.float(), 64, 32), lambda: hip_ops.dequantize_w4(wq, scales[:1], 64, 32),
+                lambda: hip_ops.dequantize_w4(wq[:, :, :32], scales, 64, 32), lambda: hip_ops.linear_w4(torch.zeros(1, 64), wq, scales, 32)):
+        with pytest.raises(ValueError):
+            bad()
+    layer = autograd.LinearW4.from_linear(autograd.Linear(64, 32))
+    with pytest.raises(ValueError, match="CUDA"):
+        layer(torch.zeros(1, 64))
+    again = autograd.LinearW4(64, 32)
+    again.load_state_dict(layer.state_dict())
+    assert torch.equal(again.wq, layer.wq) and torch.equal(again.scales.view(torch.int16), layer.scales.view(torch.int16))
+
+
+def test_the_native_side_refuses_bad_blocks():
+    from distributed_tensorflow_amd import native
+    from distributed_tensorflow_amd.ops import hip_ops
+    lib = native.hip()
+    assert lib.dtf_sizeof_linear_w4_args() == ctypes.sizeof(hip_ops.LinearW4Args)
+    a = hip_ops.LinearW4Args()
+    assert lib.dtf_linear_w4(None, None) == -22 and lib.dtf_linear_w4(ctypes.byref(a), None) == -22
+    a.x = a.wq = a.scales = a.y = 64
+    a.M = a.N = a.K = 1
+    for group, xtype, rows, wq in ((16, 0, 1, 64), (32, 3, 1, 64), (32, 0, 0, 64), (32, 0, 1 << 40, 64), (32, 0, 1, 72)):
+        a.group, a.xtype, a.M, a.wq = group, xtype, rows, wq
+        assert lib.dtf_linear_w4(ctypes.byref(a), None) == -22

@@ -1,0 +1,160 @@
+"""csrc/hip/linear_w4.hip through ops.hip_ops, against float64 products with the weights that the codes stand for."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+F, B, E = torch.float32, torch.bfloat16, torch.float8_e4m3fn
+U = 2.0 ** -24
+
+
+def _weights(K, N, group, seed=0):
+    from distributed_tensorflow_amd.ops import hip_ops
+    gen = torch.Generator("cuda").manual_seed(seed)
+    w = torch.randn(K, N, generator=gen, device="cuda") * torch.exp(torch.randn(1, N, generator=gen, device="cuda"))
+    wq, scales = hip_ops.quantize_w4(w, group)
+    return wq, scales, hip_ops.dequantize_w4(wq, scales, K, N).double()
+
+
+def _rows(M, K, dtype, seed=1):
+    gen = torch.Generator("cuda").manual_seed(seed)
+    x = torch.randn(M, K, generator=gen, device="cuda") * torch.exp(2 * torch.randn(M, 1, generator=gen, device="cuda"))
+    if dtype != E:
+        return x.to(dtype), None
+    scale = x.abs().amax(1) / 448
+    return (x / scale[:, None]).to(E), scale
+
+
+def check(y, x, scale, w, bias, relu):
+    """Products of bf16 parts are exact in fp32.  A sum of K of them, its groups' and waves' partial sums: no more than K + 100 additions of
+    U each on the magnitudes (three parts of an fp32 row: within 1.01 of its own), then scale, bias and the result's type."""
+    x = x.double() if scale is None else x.double() * scale.double()[:, None]
+    want, size = x @ w, x.abs() @ w.abs()
+    K = x.shape[1]
+    off = size * (3 * K + 100) * U
+    if bias is not None:
+        want, off = want + bias.double(), off + U * (want.abs() + bias.double().abs()) * 2
+    if relu:
+        want = want.clamp(min=0)
+    off = off + want.abs() * (2.0 ** -8 if y.dtype == B else U) + 1e-37
+    worst = ((y.double() - want).abs() / off).max()
+    assert bool(worst <= 1), float(worst)
+
+
+# (rows, K, N): one element; tails of k and of outputs; one k tile and many; one, two and four tiles of columns; rows behind the last chunk
+SHAPES = [(1, 1, 1), (1, 128, 16), (1, 2048, 1008), (2, 130, 33), (3, 127, 5), (5, 3136, 1025), (6, 96, 40), (10, 256, 48), (11, 264, 16), (16, 512, 64),
+          (17, 1000, 31), (32, 1024, 16), (33, 72, 100), (64, 640, 200), (65, 256, 17), (150, 136, 20), (1, 16384, 8200), (16, 4096, 8208)]
+
+
+@pytest.mark.parametrize("dtype", [F, B, E])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,K,N", SHAPES)
+def test_products(M, K, N, group, dtype):
+    from distributed_tensorflow_amd.ops import hip_ops
+    wq, scales, w = _weights(K, N, group)
+    x, scale = _rows(M, K, dtype)
+    bias = torch.randn(N, generator=torch.Generator("cuda").manual_seed(2), device="cuda")
+    y = hip_ops.linear_w4(x, wq, scales, N, bias=bias, x_scale=scale)
+    check(y, x, scale, w, bias, False)
+    assert torch.equal(y, hip_ops.linear_w4(x, wq, scales, N, bias=bias, x_scale=scale))  # a fixed order of the sums
+    check(hip_ops.linear_w4(x, wq, scales, N, relu=True, x_scale=scale, out_dtype=B), x, scale, w, None, True)
+
+
+@pytest.mark.parametrize("dtype", [F, B, E])
+@pytest.mark.parametrize("K", [256, 257, 264])
+def test_strides_alignment_and_leading_dimensions(K, dtype):
+    from distributed_tensorflow_amd.ops import hip_ops
+    wq, scales, w = _weights(K, 40, 32)
+    wide, scale = _rows(7, K + 50, dtype)
+    for lo in (0, 1, 2, 8, 16):
+        x = wide[:, lo:lo + K]
+        check(hip_ops.linear_w4(x, wq, scales, 40, x_scale=scale), x, scale, w, None, False)
+    t = wide[:, :K].t().contiguous().t()  # elements of a row apart from one another
+    check(hip_ops.linear_w4(t, wq, scales, 40, x_scale=scale), t, scale, w, None, False)
+    y = hip_ops.linear_w4(wide[:6, :K].reshape(2, 3, K), wq, scales, 40, x_scale=None if scale is None else scale[:6])
+    assert y.shape == (2, 3, 40)
+    check(y.reshape(6, 40), wide[:6, :K], None if scale is None else scale[:6], w, None, False)
+    one = hip_ops.linear_w4(wide[0, :K].contiguous(), wq, scales, 40, x_scale=None if scale is None else scale[:1])
+    assert one.shape == (40,) and torch.equal(one, hip_ops.linear_w4(wide[:1, :K], wq, scales, 40, x_scale=None if scale is None else scale[:1])[0])
+    if dtype != E:  # one row for all, and a scale that other types may have
+        e = wide[:1, :K].expand(5, K)
+        s = torch.rand(5, device="cuda")
+        check(hip_ops.linear_w4(e, wq, scales, 40, x_scale=s), e, s, w, None, False)
+
+
+def test_float32_rows_lose_nothing_to_the_matrix_instructions_type():
+    """A single weight of 1: the output is x itself, all 24 bits of it, far down the range of exponents."""
+    from distributed_tensorflow_amd.ops import hip_ops
+    w = torch.zeros(64, 16)
+    w[5, 3] = 6.0
+    wq, scales = (t.cuda() for t in hip_ops.quantize_w4(w, 32))
+    gen = torch.Generator("cuda").manual_seed(0)
+    for e in (0, 100, -60, -90):
+        x = torch.zeros(5, 64, device="cuda")
+        x[:, 5] = torch.randn(5, generator=gen, device="cuda") * 2.0 ** e
+        y = hip_ops.linear_w4(x, wq, scales, 16)
+        assert torch.equal(y[:, 3].double(), (x[:, 5].double() * 6).float().double())
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+def test_infinities_and_nan_stay_in_their_rows(dtype):
+    from distributed_tensorflow_amd.ops import hip_ops
+    wq, scales, w = _weights(200, 20, 64)
+    w4 = w.float()
+    assert bool((w4 != 0).any())
+    x, _ = _rows(5, 200, dtype)
+    x[1, 7], x[2, 199], x[3, 0] = float("inf"), float("nan"), -float("inf")
+    x[4] = 0
+    y = hip_ops.linear_w4(x, wq, scales, 20)
+    check(y[:1], x[:1], None, w, None, False)
+    assert bool(torch.isnan(y[2]).all()) and not y[4].any()
+    for row, k, sign in ((1, 7, 1), (3, 0, -1)):
+        want = w4[k] * sign * float("inf")  # a weight of zero gives NaN
+        assert torch.equal(torch.isnan(want), torch.isnan(y[row])) and torch.equal(want[w4[k] != 0], y[row][w4[k] != 0])
+    relu = hip_ops.linear_w4(x, wq, scales, 20, relu=True)
+    assert bool(torch.isnan(relu[2]).all())
+    if dtype == F:  # a NaN whose payload lies in the low bits alone
+        z = torch.zeros(1, 200, device="cuda")
+        z.view(torch.int32)[0, 3] = 0x7F800001
+        assert bool(torch.isnan(hip_ops.linear_w4(z, wq, scales, 20)).all())
+
+
+def test_layers_capture_and_another_stream():
+    from distributed_tensorflow_amd.ops import autograd
+    layer = autograd.Linear(256, 100, relu=True).cuda()
+    q = autograd.LinearW4.from_linear(layer, 32)
+    from distributed_tensorflow_amd.ops import hip_ops
+    w = hip_ops.dequantize_w4(q.wq, q.scales, 256, 100).double()
+    x = _rows(3, 256, F)[0]
+    check(q(x), x, None, w, layer.bias.detach(), True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = q(x)
+    for i in range(4):
+        x.copy_(_rows(3, 256, F, seed=i + 5)[0])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, q(x))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        z = q(x)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(y, z)
+
+
+def test_empty_batches_and_refusals():
+    from distributed_tensorflow_amd.ops import hip_ops
+    wq, scales, _ = _weights(64, 32, 64)
+    x = torch.zeros(2, 64, device="cuda")
+    assert hip_ops.linear_w4(x[:0], wq, scales, 32).shape == (0, 32)
+    for bad in (lambda: hip_ops.linear_w4(x.half(), wq, scales, 32), lambda: hip_ops.linear_w4(x.to(E), wq, scales, 32),
+                lambda: hip_ops.linear_w4(torch.zeros(2, 129, device="cuda"), wq, scales, 32), lambda: hip_ops.linear_w4(x, wq, scales, 33),
+                lambda: hip_ops.linear_w4(x, wq, scales, 16), lambda: hip_ops.linear_w4(x, wq.cpu(), scales.cpu(), 32),
+                lambda: hip_ops.linear_w4(x, wq, scales, 32, bias=torch.zeros(31, device="cuda")),
+                lambda: hip_ops.linear_w4(x, wq, scales, 32, bias=torch.zeros(32, device="cuda", dtype=B)),
+                lambda: hip_ops.linear_w4(x, wq, scales, 32, x_scale=torch.zeros(1, device="cuda")),
+                lambda: hip_ops.linear_w4(x, wq, scales, 32, out_dtype=torch.float16),
+                lambda: hip_ops.linear_w4(x[:, :0], wq, scales, 32),
+                lambda: hip_ops.linear_w4(x[:1].expand(hip_ops.W4_MAX_ROWS + 1, 64), wq, scales, 32)):
+        with pytest.raises(ValueError):
+            bad()
