@@ -1,5 +1,6 @@
-// What a launch of AdamW takes (mirrored by distributed_tensorflow_amd/optim/adamw.py).
+// What a launch of AdamW takes.
 #pragma once
+#include <hip/hip_runtime_api.h>
 #include <stdint.h>
 
 struct AdamWLaunch {
@@ -18,3 +19,9 @@ struct AdamWLaunch {
   uint32_t seed;
   int ntensors, nchunks, bits;
 };
+
+// Bytes of `live` for each tensor.
+extern "C" int dtf_sizeof_adamw_live();
+// p, g, kind: host arrays of a->ntensors entries (g = 0: the tensor takes no part in this step; kind: bit 0 bf16 parameters, bit 1
+// bf16 gradients)
+extern "C" int dtf_adamw(const AdamWLaunch* a, const uint64_t* p, const uint64_t* g, const uint8_t* kind, hipStream_t st);

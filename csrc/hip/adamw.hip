@@ -219,11 +219,8 @@ template <typename P, typename G> static void adamw_apply(const AdamWLaunch& a, 
   else hipLaunchKernelGGL((adamw_apply_kernel<P, G, false>), dim3(a.nchunks), dim3(256), 0, st, a);
 }
 
-DTF_API int dtf_sizeof_adamw_launch() { return (int)sizeof(AdamWLaunch); }
 DTF_API int dtf_sizeof_adamw_live() { return (int)sizeof(AdamWLive); }
 
-// p, g, kind: host arrays of a->ntensors entries (g = 0: the tensor takes no part in this step; kind: bit 0 bf16 parameters, bit 1
-// bf16 gradients)
 DTF_API int dtf_adamw(const AdamWLaunch* a, const uint64_t* p, const uint64_t* g, const uint8_t* kind, hipStream_t st) {
   if (!a || !p || !g || !kind || a->ntensors < 0 || a->nchunks < 0 || (a->bits != 8 && a->bits != 32)) return -22;
   if (a->ntensors == 0 || a->nchunks == 0) return 0;

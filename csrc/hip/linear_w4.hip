@@ -13,23 +13,12 @@
 // The waves of a workgroup split k (tile t goes to wave t mod waves, so that the workgroup streams contiguously) and add their partial
 // results in LDS, in the waves' order.
 #include "common.h"
+#include "linear_w4.h"
 
 namespace {
 constexpr int ERR = -22;
 }
 
-struct LinearW4Args {  // mirrored by distributed_tensorflow_amd/ops/hip_ops.py
-  const void* x;         // [M][ldx]
-  const void* wq;        // [Nt][Kt][64][16] bytes, Nt = ceil(N / 16), Kt = ceil(K / 128)
-  const uint16_t* scales;// bf16 [Nt][Kt * 128 / G][16]
-  const float* bias;     // [N] or null
-  const float* x_scale;  // [M] or null
-  void* y;               // [M][N] fp32 or bf16
-  long M, ldx;
-  int N, K, group, xtype, relu, out_bf16;  // xtype: 0 fp32, 1 bf16, 2 e4m3
-};
-
-enum { X_F32 = 0, X_BF16 = 1, X_E4M3 = 2 };
 template <int XT> struct XType { using T = float; static constexpr int P = 3; };  // P: columns of B a row takes
 template <> struct XType<X_BF16> { using T = uint16_t; static constexpr int P = 1; };
 template <> struct XType<X_E4M3> { using T = uint8_t; static constexpr int P = 1; };
@@ -220,8 +209,6 @@ template <int XT> void with_rows(const LinearW4Args& a, hipStream_t st) {
   else with_group<XT, false>(a, st);
 }
 }  // namespace
-
-DTF_API int dtf_sizeof_linear_w4_args() { return (int)sizeof(LinearW4Args); }
 
 DTF_API int dtf_linear_w4(const LinearW4Args* p, hipStream_t st) {
   if (!p || !p->x || !p->wq || !p->scales || !p->y || p->M <= 0 || p->N <= 0 || p->K <= 0 || p->ldx < 0) return ERR;

@@ -9,30 +9,13 @@
 // dw: every workgroup of the backward pass adds up its rows in registers and writes one row of partial sums; a second kernel adds
 // those in a fixed order (no atomics: the same result on every run).
 #include "common.h"
+#include "rms_norm.h"
 
 namespace {
 constexpr int ERR = -22;
 constexpr float E4M3_MAX = 448.f;
 constexpr float TINY = 0x1p-100f;  // a row whose largest magnitude is below this is scaled as if it were this: 448 / max stays finite
 }  // namespace
-
-struct RmsNormArgs {  // mirrored by distributed_tensorflow_amd/ops/hip_ops.py
-  const void* x;
-  const void* res;    // or null
-  const void* dy;     // backward only, as dh (or null: h has no gradient of its own)
-  const void* dh;
-  const float* w;
-  void* y;            // output rows, contiguous: fp32 / bf16, or e4m3 where q_scale is given; backward: dx
-  void* h;            // x + res (only with res)
-  float* rstd;        // forward: written unless null
-  float* q_scale;
-  float* part;        // backward: [blocks][dim] partial sums of dw, or null
-  float* dw;
-  long rows, ld_x, ld_res, ld_dy, ld_dh;
-  int dim, bf16;
-  float eps;
-  int blocks;         // backward: rows of `part`
-};
 
 template <typename T, int VEC> struct Piece {  // VEC consecutive elements as loaded (T: float, or uint16_t for bf16)
   T e[VEC];
@@ -388,8 +371,6 @@ bool bad(const RmsNormArgs* a) {
   return !a || !a->x || !a->w || !a->y || a->rows <= 0 || a->dim <= 0 || a->rows > 0x7fffffffL || a->ld_x < 0 || a->ld_res < 0 || a->ld_dy < 0 || a->ld_dh < 0;
 }
 }  // namespace
-
-DTF_API int dtf_sizeof_rms_norm_args() { return (int)sizeof(RmsNormArgs); }
 
 DTF_API int dtf_rms_norm_fwd(const RmsNormArgs* p, hipStream_t st) {
   if (bad(p) || (p->res && !p->h)) return ERR;

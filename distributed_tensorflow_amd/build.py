@@ -3,6 +3,8 @@
 * ``csrc/hip/*.hip``  -> ``distributed_tensorflow_amd/_lib/libdtf_hip.so``  (hipcc, ``--offload-arch=gfx950`` only)
 * ``csrc/host/*.cc``  -> ``distributed_tensorflow_amd/_lib/libdtf_host.so`` (g++; tfevents writer, CRC32C,
   TCP rendezvous store, checkpoint container, IDX/bottleneck text codecs)
+* ``csrc/torch/*.cc`` -> ``distributed_tensorflow_amd/_lib/libdtf_torch.so`` (g++ against torch's headers; entry points on torch
+  tensors over libdtf_hip.so, a Python module)
 
 hipcc cross-compiles without a GPU, so the build also runs on the CPU-only CI box; the resulting
 ``.so`` files are git-ignored but travel with the tree to the GPU box.
@@ -15,6 +17,7 @@ import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from typing import List
 
@@ -70,7 +73,12 @@ def _sources(srcdir: str, exts) -> List[str]:
 def source_digest(which: str) -> str:
     """Digest of the sources + build line that ``libdtf_<which>.so`` must have been built from."""
     srcdir, exts, cc, ld, _ = _recipe(which)
-    return _digest(_sources(srcdir, exts) + _headers(srcdir), " ".join(cc + ld))
+    return _digest(_sources(srcdir, exts) + _all_headers(which), " ".join(cc + ld))
+
+
+def _all_headers(which: str) -> List[str]:
+    # (the torch entry points include the argument blocks of csrc/hip)
+    return _headers(os.path.join(CSRC, "hip" if which == "torch" else which))
 
 
 def is_current(which: str) -> bool:
@@ -84,7 +92,7 @@ def _build_lib(which: str, force: bool, jobs: int) -> str:
         raise RuntimeError("no sources in " + srcdir)
     os.makedirs(LIBDIR, exist_ok=True)
     os.makedirs(OBJDIR, exist_ok=True)
-    digest = _digest(srcs + _headers(srcdir), " ".join(compiler_cmd + link_cmd))
+    digest = source_digest(which)
     if not force and os.path.exists(out) and embedded_digest(out) == digest:
         return out
     # the digest travels inside the library (dtf_<which>_source_digest()), not in a side-car file that can go stale
@@ -114,6 +122,17 @@ def _recipe(which: str):
         cc += os.environ.get("DTF_EXTRA_HIPCC_FLAGS", "").split()  # (experiments; part of the digest)
         ld = [HIPCC, "--offload-arch=" + ARCH, "-shared", "-fPIC"]
         return d, (".hip",), cc, ld, os.path.join(LIBDIR, "libdtf_hip.so")
+    if which == "torch":
+        import torch
+        d, home = os.path.join(CSRC, "torch"), os.path.dirname(torch.__file__)
+        rocm = os.path.dirname(os.path.dirname(HIPCC))
+        cc = [CXX, "-O2", "-fPIC", "-std=c++17", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"]
+        for i in (home + "/include", home + "/include/torch/csrc/api/include", rocm + "/include", sysconfig.get_paths()["include"]):
+            cc += ["-isystem", i]
+        cc += ["-I", os.path.join(CSRC, "hip")]
+        ld = [CXX, "-shared", "-fPIC", "-Wl,--no-as-needed", "-L", LIBDIR, "-l:libdtf_hip.so", "-Wl,-rpath,$ORIGIN", "-L", home + "/lib", "-ltorch", "-ltorch_cpu",
+              "-ltorch_python", "-ltorch_hip", "-lc10", "-lc10_hip"]
+        return d, (".cc",), cc, ld, os.path.join(LIBDIR, "libdtf_torch.so")
     d = os.path.join(CSRC, "host")
     cc = [CXX, "-O2", "-fPIC", "-std=c++17", "-fvisibility=hidden", "-pthread", "-I", d]
     ld = [CXX, "-shared", "-fPIC", "-pthread"]
@@ -126,6 +145,11 @@ def build_hip(force: bool = False, jobs: int = 4) -> str:
 
 def build_host(force: bool = False, jobs: int = 4) -> str:
     return _build_lib("host", force, jobs)
+
+
+def build_torch(force: bool = False, jobs: int = 4) -> str:
+    build_hip()
+    return _build_lib("torch", force, jobs)
 
 
 SANITIZERS = {
@@ -149,7 +173,7 @@ def build_host_selftest(sanitizer: str = "", outdir: str = "") -> str:
 
 
 def build_all(force: bool = False) -> List[str]:
-    return [build_host(force), build_hip(force)]
+    return [build_host(force), build_hip(force), build_torch(force)]
 
 
 if __name__ == "__main__":

@@ -1,6 +1,7 @@
 """ctypes bindings to the in-tree native libraries.
 
 * ``hip()``  -> ``_lib/libdtf_hip.so``  (gfx950 kernels + step executor; needs a GPU to *run*, loads anywhere ROCm is installed)
+* ``ext()``  -> ``_lib/libdtf_torch.so`` (a Python module: entry points that take torch tensors, over libdtf_hip.so)
 * ``host()`` -> ``_lib/libdtf_host.so`` (CRC32C, tfevents writer, rendezvous store, checkpoint container)
 
 There is deliberately no silent fallback: if a library is missing it is built on the spot
@@ -18,6 +19,7 @@ _LIBDIR = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib")
 _lock = threading.Lock()
 _hip: Optional[C.CDLL] = None
 _host: Optional[C.CDLL] = None
+_ext = None
 
 c_void_p, c_int, c_long, c_float, c_uint64, c_int64, c_char_p = (
     C.c_void_p, C.c_int, C.c_long, C.c_float, C.c_uint64, C.c_int64, C.c_char_p)
@@ -81,13 +83,13 @@ class MnistEngineStruct(C.Structure):  # csrc/hip/engine.hip: struct MnistEngine
 def _ensure_built(name: str) -> str:
     path = os.path.join(_LIBDIR, name)
     from . import build
-    which = "hip" if "hip" in name else "host"
+    which = "hip" if "hip" in name else "torch" if "torch" in name else "host"
     stale = os.path.exists(path) and os.path.isdir(build.CSRC) and not build.is_current(which)
     if stale and os.environ.get("DTF_ALLOW_STALE_LIB", "0") == "1":
         stale = False
     if not os.path.exists(path) or stale:
         # (a library that was not built from the sources next to it is rebuilt, never used silently)
-        (build.build_hip if which == "hip" else build.build_host)()
+        {"hip": build.build_hip, "torch": build.build_torch, "host": build.build_host}[which]()
     if not os.path.exists(path):
         raise NativeError("native library %s is missing and could not be built" % path)
     return path
@@ -288,6 +290,22 @@ def host() -> C.CDLL:
         _sig(lib, "dtf_format_floats", c_int64, [P, c_uint64, P, c_uint64])
         _host = lib
         return lib
+
+
+def ext():
+    """The module of ``csrc/torch/bindings.cc``; it uses the library that ``hip()`` has loaded."""
+    global _ext
+    if _ext is None:
+        hip()
+        with _lock:
+            if _ext is None:
+                import importlib.machinery
+                import importlib.util
+                loader = importlib.machinery.ExtensionFileLoader("libdtf_torch", _ensure_built("libdtf_torch.so"))
+                module = importlib.util.module_from_spec(importlib.util.spec_from_loader("libdtf_torch", loader))
+                loader.exec_module(module)
+                _ext = module
+    return _ext
 
 
 def check(rc: int, what: str) -> None:

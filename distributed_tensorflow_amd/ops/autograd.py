@@ -21,7 +21,6 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from .. import native
 from . import hip_ops
@@ -238,29 +237,10 @@ def avg_pool3x3_same(x: torch.Tensor) -> torch.Tensor:
     return _AvgPool3x3Same.apply(x)
 
 
-class _RMSNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps: float):
-        y, h, rstd = hip_ops.rms_norm_forward(x, weight, residual, eps)
-        ctx.save_for_backward(x, rstd, weight, residual)
-        ctx.set_materialize_grads(False)
-        return y if residual is None else (y, h)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh=None):
-        x, rstd, weight, residual = ctx.saved_tensors
-        need_x, need_w, need_r, _ = ctx.needs_input_grad
-        if dy is None:  # only h went into the loss
-            return dh if need_x else None, torch.zeros_like(weight) if need_w else None, dh if need_r else None, None
-        dx, dw = hip_ops.rms_norm_backward(dy, x, rstd, weight, residual, dh, need_dw=need_w)
-        return dx if need_x else None, dw, dx if need_r else None, None
-
-
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
     """``h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension; ``y``, or ``(y, h)`` with a residual.
     ``x`` and ``residual`` fp32 or bf16 of one shape and type, ``weight`` fp32; differentiable once in all three."""
-    return _RMSNorm.apply(x, weight, residual, eps)
+    return native.ext().rms_norm(x, weight, residual, eps)
 
 
 # ------------------------------------------------------------------------------------------------ layers

@@ -323,82 +323,14 @@ def conv2_backward_f32(dpool2: torch.Tensor, pool2: torch.Tensor, amax2: torch.T
     return dpool1, dW, db
 
 
-# ----------------------------------------------------------------------------- RMS norm (csrc/hip/rms_norm.hip)
-class RmsNormArgs(C.Structure):  # csrc/hip/rms_norm.hip
-    _fields_ = [("x", C.c_void_p), ("res", C.c_void_p), ("dy", C.c_void_p), ("dh", C.c_void_p), ("w", C.c_void_p), ("y", C.c_void_p), ("h", C.c_void_p),
-                ("rstd", C.c_void_p), ("q_scale", C.c_void_p), ("part", C.c_void_p), ("dw", C.c_void_p),
-                ("rows", C.c_long), ("ld_x", C.c_long), ("ld_res", C.c_long), ("ld_dy", C.c_long), ("ld_dh", C.c_long),
-                ("dim", C.c_int), ("bf16", C.c_int), ("eps", C.c_float), ("blocks", C.c_int)]
-
-
-native.register_hip_sig("dtf_sizeof_rms_norm_args", C.c_int, [])
-native.register_hip_sig("dtf_rms_norm_fwd", C.c_int, [C.POINTER(RmsNormArgs), C.c_void_p])
-native.register_hip_sig("dtf_rms_norm_bwd_blocks", C.c_int, [C.c_long, C.c_int])
-native.register_hip_sig("dtf_rms_norm_bwd", C.c_int, [C.POINTER(RmsNormArgs), C.c_void_p])
-
-
-def _launch(t: torch.Tensor, what: str, fn, *args) -> None:
-    """``fn(*args, stream)`` on the current stream of the device that ``t`` is on."""
-    if t.device.index == torch.cuda.current_device():
-        native.check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
-    else:
-        with torch.cuda.device(t.device):
-            native.check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
-
-
-def _rows(t: torch.Tensor, like: Optional[torch.Tensor], name: str) -> Tuple[torch.Tensor, int]:
-    """``t`` as rows of its last dimension, and the rows' stride: any stride between rows, none inside one (else a copy)."""
-    if not t.is_cuda or t.dtype not in (torch.float32, torch.bfloat16) or t.dim() < 1:
-        raise ValueError("%s must be a CUDA tensor of float32 or bfloat16 rows (got %s, cuda=%s, shape %s)"
-                         % (name, t.dtype, t.is_cuda, tuple(t.shape)))
-    if like is not None and (t.dtype != like.dtype or t.shape != like.shape or t.device != like.device):
-        raise ValueError("%s (%s %s on %s) must have the type, shape and device of the other rows (%s %s on %s)"
-                         % (name, t.dtype, tuple(t.shape), t.device, like.dtype, tuple(like.shape), like.device))
-    if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1]) if t.numel() else t.new_empty(0, t.shape[-1])
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        t = t.contiguous()
-    return t, t.stride(0)
-
-
-def _norm_weight(weight: torch.Tensor, x: torch.Tensor, eps: float) -> None:
-    _chk(weight, torch.float32, "weight")
-    if weight.dim() != 1 or weight.device != x.device or x.dim() < 1 or x.shape[-1] != weight.shape[0] or weight.shape[0] < 1:
-        raise ValueError("weight %s on %s does not fit rows of shape %s on %s" % (tuple(weight.shape), weight.device, tuple(x.shape), x.device))
-    if not eps >= 0:
-        raise ValueError("eps must not be negative (got %r)" % (eps,))
-
-
-def _rms_norm(x, weight, residual, eps, eight: bool):
-    x2, ld_x = _rows(x, None, "x")
-    _norm_weight(weight, x, eps)
-    a = RmsNormArgs()
-    h = x
-    if residual is not None:
-        r2, a.ld_res = _rows(residual, x, "residual")
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        a.res, a.h = r2.data_ptr(), h.data_ptr()
-    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if eight else x.dtype, device=x.device)
-    side = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)  # the rows' scales, or their rstd
-    if x.numel():
-        a.x, a.ld_x, a.w, a.y = x2.data_ptr(), ld_x, weight.data_ptr(), y.data_ptr()
-        if eight:
-            a.q_scale = side.data_ptr()
-        else:
-            a.rstd = side.data_ptr()
-        a.rows, a.dim, a.bf16, a.eps = x2.shape[0], x2.shape[1], x.dtype == torch.bfloat16, eps
-        _launch(x, "rms_norm_fwd", native.hip().dtf_rms_norm_fwd, C.byref(a))
-    return y, side, h
-
-
+# ----------------------------------------------------------------------------- RMS norm (csrc/hip/rms_norm.hip, csrc/torch/bindings.cc)
 def rms_norm_forward(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6
                      ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension -> ``(y, h, rstd)``.
 
     ``x``, ``residual``: fp32 or bf16 rows of one type, any stride between rows; ``weight`` fp32.  ``h`` (``x`` itself without a
     residual) is rounded to that type, ``y`` comes from the unrounded sum; ``rstd`` (fp32, one a row) is for ``rms_norm_backward``."""
-    y, rstd, h = _rms_norm(x, weight, residual, eps, False)
-    return y, h, rstd
+    return native.ext().rms_norm_forward(x, weight, residual, eps)
 
 
 def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6
@@ -406,56 +338,18 @@ def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torc
     """The same with an output in 8 bits, for inference: ``(q, scale, h)``, ``y ~ q * scale``; ``q`` e4m3 and ``scale`` fp32, one a
     row: its largest magnitude / 448.  A row of zeros has the scale 0, one that holds a NaN the scale NaN; a row whose largest magnitude is
     below 2^-100 is scaled as if that were it."""
-    return _rms_norm(x, weight, residual, eps, True)
+    return native.ext().rms_norm_e4m3(x, weight, residual, eps)
 
 
 def rms_norm_backward(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
                       dh: Optional[torch.Tensor] = None, need_dw: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``(dx, dw)`` of ``rms_norm_forward``; ``dx`` is the residual's gradient too.  ``dh``: the gradient that ``h`` has from elsewhere.
     ``dw`` is summed in a fixed order: the same bits on every run."""
-    x2, ld_x = _rows(x, None, "x")
-    _norm_weight(weight, x, 0.0)
-    d2, ld_d = _rows(dy, x, "dy")
-    _chk(rstd, torch.float32, "rstd")
-    if rstd.shape != x.shape[:-1] or rstd.device != x.device:
-        raise ValueError("rstd %s on %s does not fit rows of shape %s on %s" % (tuple(rstd.shape), rstd.device, tuple(x.shape), x.device))
-    a = RmsNormArgs()
-    if residual is not None:
-        r2, a.ld_res = _rows(residual, x, "residual")
-        a.res = r2.data_ptr()
-    if dh is not None:
-        g2, a.ld_dh = _rows(dh, x, "dh")
-        a.dh = g2.data_ptr()
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    rows, dim = x2.shape
-    if not x.numel():
-        return dx, torch.zeros_like(weight) if need_dw else None
-    lib = native.hip()
-    blocks = lib.dtf_rms_norm_bwd_blocks(rows, dim)
-    dw = None
-    if need_dw:
-        dw = torch.empty_like(weight)
-        part = torch.empty(blocks, dim, dtype=torch.float32, device=x.device)
-        a.part, a.dw = part.data_ptr(), dw.data_ptr()
-    a.x, a.ld_x, a.dy, a.ld_dy, a.w, a.y, a.rstd = x2.data_ptr(), ld_x, d2.data_ptr(), ld_d, weight.data_ptr(), dx.data_ptr(), rstd.data_ptr()
-    a.rows, a.dim, a.bf16, a.blocks = rows, dim, x.dtype == torch.bfloat16, blocks
-    _launch(x, "rms_norm_bwd", lib.dtf_rms_norm_bwd, C.byref(a))
-    return dx, dw
+    return native.ext().rms_norm_backward(dy, x, rstd, weight, residual, dh, need_dw)
 
 
 # ----------------------------------------------------------------------------- dense layers with 4-bit weights (csrc/hip/linear_w4.hip)
-class LinearW4Args(C.Structure):  # csrc/hip/linear_w4.hip
-    _fields_ = [("x", C.c_void_p), ("wq", C.c_void_p), ("scales", C.c_void_p), ("bias", C.c_void_p), ("x_scale", C.c_void_p),
-                ("y", C.c_void_p), ("M", C.c_long), ("ldx", C.c_long), ("N", C.c_int), ("K", C.c_int), ("group", C.c_int),
-                ("xtype", C.c_int), ("relu", C.c_int), ("out_bf16", C.c_int)]
-
-
-native.register_hip_sig("dtf_sizeof_linear_w4_args", C.c_int, [])
-native.register_hip_sig("dtf_linear_w4", C.c_int, [C.POINTER(LinearW4Args), C.c_void_p])
-
 _E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
-_X_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float8_e4m3fn: 2}
-W4_MAX_ROWS = 65535 * 5
 
 
 def quantize_w4(w: torch.Tensor, group: int = 64) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -519,32 +413,6 @@ def linear_w4(x: torch.Tensor, wq: torch.Tensor, scales: torch.Tensor, out_featu
     ``x[..., K]`` fp32 (not rounded), bf16, or e4m3 with ``x_scale`` (fp32, one a row; as ``rms_norm_e4m3`` gives them; optional for
     the other types); any stride between rows.  ``bias`` fp32 ``[out_features]``; the result fp32 or bf16 ``[..., out_features]``.  Sums are fp32.
     More than 64 rows (fp32: 10) read the weights again for each further 64."""
-    group = _w4_group(wq, scales)
-    if not x.is_cuda or x.dtype not in _X_TYPES or x.dim() < 1 or x.device != wq.device:
-        raise ValueError("x must be a CUDA tensor of float32, bfloat16 or float8_e4m3fn on the weights' device (got %s on %s)" % (x.dtype, x.device))
-    K, N = x.shape[-1], int(out_features)
-    if K < 1 or -(-K // 128) != wq.shape[1] or N < 1 or -(-N // 16) != wq.shape[0]:
-        raise ValueError("x %s and %d outputs do not fit weights of %d x %d tiles of 128 x 16" % (tuple(x.shape), N, wq.shape[1], wq.shape[0]))
     if out_dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("out_dtype is float32 or bfloat16 (got %s)" % (out_dtype,))
-    if x_scale is None and x.dtype == torch.float8_e4m3fn:
-        raise ValueError("e4m3 rows need their x_scale")
-    for t, name, n in ((bias, "bias", N), (x_scale, "x_scale", x.numel() // K)):
-        if t is not None:
-            _chk(t, torch.float32, name)
-            if t.numel() != n or t.device != x.device:
-                raise ValueError("%s has %d elements on %s, not %d on %s" % (name, t.numel(), t.device, n, x.device))
-    y = torch.empty(x.shape[:-1] + (N,), dtype=out_dtype, device=x.device)
-    if not x.numel():
-        return y
-    x2 = x if x.dim() == 2 else x.reshape(-1, K)
-    if K > 1 and x2.stride(1) != 1:
-        x2 = x2.contiguous()
-    if x2.shape[0] > W4_MAX_ROWS:
-        raise ValueError("at most %d rows (got %d)" % (W4_MAX_ROWS, x2.shape[0]))
-    a = LinearW4Args()
-    a.x, a.wq, a.scales, a.bias, a.x_scale, a.y = x2.data_ptr(), wq.data_ptr(), scales.data_ptr(), native.ptr(bias), native.ptr(x_scale), y.data_ptr()
-    a.M, a.ldx, a.N, a.K, a.group, a.xtype = x2.shape[0], x2.stride(0), N, K, group, _X_TYPES[x.dtype]
-    a.relu, a.out_bf16 = relu, out_dtype == torch.bfloat16
-    _launch(x, "linear_w4", native.hip().dtf_linear_w4, C.byref(a))
-    return y
+    return native.ext().linear_w4(x, wq, scales, out_features, bias, relu, x_scale, out_dtype == torch.bfloat16)

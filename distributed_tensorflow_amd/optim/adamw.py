@@ -18,8 +18,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from array import array
-from typing import Dict, Iterable, List, Optional, Sequence
+from typing import Dict, Iterable, Optional, Sequence
 
 import torch
 
@@ -30,17 +29,6 @@ CHUNK = 2048   # elements of a workgroup
 E4M3 = torch.float8_e4m3fn
 
 
-class AdamWLaunch(C.Structure):  # csrc/hip/adamw.h
-    _fields_ = [("shape", C.c_void_p), ("chunks", C.c_void_p), ("live", C.c_void_p), ("step", C.c_void_p), ("m", C.c_void_p),
-                ("v", C.c_void_p), ("m_scale", C.c_void_p), ("r_scale", C.c_void_p),
-                ("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double),
-                ("b1", C.c_float), ("ob1", C.c_float), ("b2", C.c_float), ("ob2", C.c_float), ("eps", C.c_float),
-                ("decay", C.c_float), ("grad_scale", C.c_float), ("seed", C.c_uint32),
-                ("ntensors", C.c_int), ("nchunks", C.c_int), ("bits", C.c_int)]
-
-
-native.register_hip_sig("dtf_adamw", C.c_int, [C.POINTER(AdamWLaunch), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p])
-native.register_hip_sig("dtf_sizeof_adamw_launch", C.c_int, [])
 native.register_hip_sig("dtf_sizeof_adamw_live", C.c_int, [])
 
 
@@ -70,19 +58,14 @@ class _Group:
             self.arenas = {"m": torch.zeros(total, dtype=torch.uint8, device=dev).view(E4M3), "m_scale": tiny,
                            "r": torch.zeros(total, dtype=torch.uint8, device=dev).view(E4M3), "r_scale": tiny.clone()}
         if self.device.type == "cuda":
-            self.kinds = bytes(int(d == torch.bfloat16) for d in self.dtypes)
             counts = torch.tensor([-(-n // CHUNK) for n in self.sizes])
             owner = torch.repeat_interleave(torch.arange(len(self.sizes)), counts)
             first = torch.cumsum(counts, 0) - counts
             self.chunks = torch.stack((owner, torch.arange(owner.numel()) - first[owner]), 1).to(torch.int32).to(dev)
             self.shape = torch.tensor(list(zip(self.sizes, self.at)), dtype=torch.int64).to(dev)
             self.live = torch.empty(len(params) * native.hip().dtf_sizeof_adamw_live(), dtype=torch.uint8, device=dev)
-            a = self.launch = AdamWLaunch()
-            a.shape, a.chunks, a.live, a.step = (t.data_ptr() for t in (self.shape, self.chunks, self.live, self.step))
-            a.m, a.v = self.arenas["m"].data_ptr(), self.arenas["v" if bits == 32 else "r"].data_ptr()
-            if bits == 8:
-                a.m_scale, a.r_scale = self.arenas["m_scale"].data_ptr(), self.arenas["r_scale"].data_ptr()
-            a.ntensors, a.nchunks, a.bits, a.seed = len(params), self.chunks.shape[0], bits, self.seed
+            places = {"shape": self.shape, "chunks": self.chunks, "live": self.live, "step": self.step, **self.arenas}
+            self.native = native.ext().AdamWGroup(self.params, {k: t.data_ptr() for k, t in places.items()}, self.chunks.shape[0], bits, self.seed)
 
     def views(self, i: int) -> Dict[str, torch.Tensor]:
         """Tensor i's part of the arenas, to the end of its last block."""
@@ -92,10 +75,13 @@ class _Group:
             out[k] = t[lo // BLOCK:hi // BLOCK] if k.endswith("scale") else t[lo:hi]
         return out
 
-    def gather(self, grads: Sequence[Optional[torch.Tensor]]) -> List[Optional[torch.Tensor]]:
-        """The gradients as the kernels take them; whatever does not fit the group is refused here, before anything is changed."""
-        out = []
-        for p, g, n, dt in zip(self.params, grads, self.sizes, self.dtypes):
+    def gather(self, given: Optional[Sequence[Optional[torch.Tensor]]]) -> bool:
+        """Takes the parameters' gradients, or the given ones; what does not fit the group is refused here, before anything is changed.
+        Whether there is one at all."""
+        if self.device.type == "cuda":
+            return self.native.gather(given)
+        self.grads = []
+        for p, g, n, dt in zip(self.params, [p.grad for p in self.params] if given is None else given, self.sizes, self.dtypes):
             if p.dtype != dt or p.numel() != n or p.device != self.device or not p.is_contiguous():
                 raise ValueError("a parameter's type, size, device or layout has changed since it was given to AdamW")
             if g is not None:
@@ -104,23 +90,16 @@ class _Group:
                 if g.device != self.device or g.shape != p.shape:
                     raise ValueError("a gradient of shape %s on %s for a parameter of shape %s on %s"
                                      % (tuple(g.shape), g.device, tuple(p.shape), self.device))
-                g = None if n == 0 else g if g.is_contiguous() else g.contiguous()
-            out.append(g)
-        return out
+            self.grads.append(g if n else None)
+        return any(g is not None for g in self.grads)
 
-    def apply(self, grads: Sequence[Optional[torch.Tensor]], o: dict, grad_scale: float) -> None:
-        if self.device.type != "cuda":
-            return self._eager(grads, o, grad_scale)
-        a = self.launch
-        a.lr, a.beta1, a.beta2 = o["lr"], o["beta1"], o["beta2"]
-        a.b1, a.ob1, a.b2, a.ob2 = o["beta1"], 1.0 - o["beta1"], o["beta2"], 1.0 - o["beta2"]
-        a.eps, a.decay, a.grad_scale = o["eps"], 1.0 - o["lr"] * o["weight_decay"], grad_scale
-        p = array("Q", [t.data_ptr() for t in self.params])
-        g = array("Q", [0 if t is None else t.data_ptr() for t in grads])
-        kinds = bytes(k if t is None or t.dtype == torch.float32 else k | 2 for k, t in zip(self.kinds, grads))
-        with torch.cuda.device(self.device):
-            native.check(native.hip().dtf_adamw(C.byref(a), p.buffer_info()[0], g.buffer_info()[0], kinds,
-                                                torch.cuda.current_stream().cuda_stream), "adamw")
+    def apply(self, o: dict, grad_scale: float) -> None:
+        """One step from the gradients that ``gather`` took."""
+        if self.device.type == "cuda":
+            self.native.launch(o["lr"], o["beta1"], o["beta2"], o["eps"], o["weight_decay"], grad_scale)
+        else:
+            grads, self.grads = self.grads, None
+            self._eager(grads, o, grad_scale)
 
     # ------------------------------------------------------------------ CPU
     def _eager(self, grads, o, grad_scale) -> None:
@@ -236,13 +215,12 @@ class AdamW(torch.optim.Optimizer):
         todo, at = [], 0
         for o, st in zip(self.param_groups, self._groups):
             if st is not None:
-                given = [p.grad for p in st.params] if grads is None else grads[at:at + len(st.params)]
+                given = None if grads is None else list(grads[at:at + len(st.params)])
                 at += len(st.params)
-                todo.append((o, st, st.gather(given)))
-        for o, st, gs in todo:
-            if any(g is not None for g in gs):
-                st.apply(gs, o, grad_scale)
-                torch.autograd.graph.increment_version([p for p, g in zip(st.params, gs) if g is not None])
+                if st.gather(given):
+                    todo.append((o, st))
+        for o, st in todo:
+            st.apply(o, grad_scale)
         return loss
 
     # ------------------------------------------------------------------ state

@@ -155,6 +155,6 @@ def test_empty_batches_and_refusals():
                 lambda: hip_ops.linear_w4(x, wq, scales, 32, x_scale=torch.zeros(1, device="cuda")),
                 lambda: hip_ops.linear_w4(x, wq, scales, 32, out_dtype=torch.float16),
                 lambda: hip_ops.linear_w4(x[:, :0], wq, scales, 32),
-                lambda: hip_ops.linear_w4(x[:1].expand(hip_ops.W4_MAX_ROWS + 1, 64), wq, scales, 32)):
+                lambda: hip_ops.linear_w4(x[:1].expand(65535 * 5 + 1, 64), wq, scales, 32)):
         with pytest.raises(ValueError):
             bad()
