@@ -92,11 +92,11 @@ template <typename T> __device__ __forceinline__ Raw8<T> raw_load(const T* src, 
   if (whole) {
 #pragma unroll
     for (int j = 0; j < (int)(sizeof(T) / 2); ++j) r.q[j] = reinterpret_cast<const uint4*>(src + e0)[j];
-  } else {  // a tensor's last elements, or one that is not aligned: inside the tensor whatever the lane
+  } else {  // a tensor's last elements, or one that is not aligned: inside the tensor whatever the lane, zeros behind it
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const long e = e0 + i < n ? e0 + i : n - 1;
-      reinterpret_cast<T*>(&r)[i] = src[e];
+      const T e = src[e0 + i < n ? e0 + i : n - 1];
+      reinterpret_cast<T*>(&r)[i] = e0 + i < n ? e : T(0);
     }
   }
   return r;
@@ -112,24 +112,33 @@ template <typename T> __device__ __forceinline__ void raw_store(T* dst, long e0,
   }
 }
 
-// The largest magnitude among the 32 lanes of a block: as bits, so that the order of the integers is that of the magnitudes.
+// The largest of the 32 lanes of a block: as bits, so that the order of the integers is that of the magnitudes.
 __device__ __forceinline__ uint32_t block_max(uint32_t x) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) x = max(x, (uint32_t)__shfl_xor((int)x, o, 64));
   return x;
 }
-__device__ __forceinline__ uint32_t finite_bits(float x) {
-  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-  return b < 0x7f800000u ? b : 0u;
+constexpr uint32_t INF_BITS = 0x7f800000u;
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t finite_magnitude(float x) { return magnitude(x) < INF_BITS ? magnitude(x) : 0u; }
+
+// The nearest float to sqrt(x) for x = 0, infinity, NaN and from 2^-96 on (every mantissa was checked): v_sqrt_f32 is at most one step off,
+// and the signs of x - (s - step) s and x - (s + step) s say which neighbour is right.  sqrtf also scales small arguments: 19 instead of
+// 9 instructions, which count here (see adamw_apply_kernel).
+__device__ __forceinline__ float sqrt_from_2_96(float x) {
+  const float s = __builtin_amdgcn_sqrtf(x), lo = __uint_as_float(__float_as_uint(s) - 1u), hi = __uint_as_float(__float_as_uint(s) + 1u);
+  const float r = fmaf(-lo, s, x) <= 0.f ? lo : s;
+  return fmaf(-hi, s, x) > 0.f ? hi : r;
 }
-// |x| * inv <= 256 to e4m3 (bias 7, three mantissa bits): adding the random bits below the kept ones and cutting rounds up with the
-// probability of the fraction.  Below 2^-6 the grid is 2^-9 throughout; one binade up a float has that grid, so 2^-6 is added there.
-__device__ __forceinline__ uint32_t stochastic_e4m3(float x, float inv, uint32_t rnd16) {
-  const float a = fabsf(x) * inv;
-  const bool low = a < 0.015625f;
-  const uint32_t u = __float_as_uint(low ? a + 0.015625f : a) + (rnd16 << 4);
-  const uint32_t code = (u >> 20) - (low ? 968u : 960u);
-  return (__float_as_uint(a) < 0x7f800000u ? code : 0x7fu) | ((__float_as_uint(x) >> 24) & 0x80u);
+// x to e4m3, |x| <= 256: v_cvt_sr_fp8_f32 adds the random bits' upper 20 below the three mantissa bits that stay and cuts (on the grid of
+// 2^-9 below 2^-6), which rounds up with the probability of the fraction.  What is not finite becomes NaN.
+__device__ __forceinline__ uint32_t stochastic_e4m3(float x, uint32_t random, uint32_t word, int byte) {
+  switch (byte) {
+    case 0: return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(x, random, (int)word, 0);
+    case 1: return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(x, random, (int)word, 1);
+    case 2: return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(x, random, (int)word, 2);
+    default: return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(x, random, (int)word, 3);
+  }
 }
 __device__ __forceinline__ void e4m3_floats(uint2 c, float* out) {
 #pragma unroll
@@ -172,32 +181,50 @@ __global__ __launch_bounds__(256) void adamw_apply_kernel(const AdamWLaunch a) {
       reinterpret_cast<float4*>(v)[h] = reinterpret_cast<const float4*>(static_cast<const float*>(a.v) + s0)[h];
     }
   }
-  uint32_t mmax = 0, rmax = 0;
+  float vmin = 1.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float g = e0 + i < l.n ? raw_get(rg, i) * a.grad_scale : 0.f;
+    const float g = raw_get(rg, i) * a.grad_scale;
     m[i] = b1 * m[i] + ob1 * g;
     v[i] = b2 * v[i] + ob2 * (g * g);
-    r[i] = sqrtf(v[i]);
-    raw_set(rp, i, raw_get(rp, i) * a.decay - l.lr1 * (m[i] / (r[i] * l.ic2 + a.eps)));
-    if constexpr (EIGHT) {
-      mmax = max(mmax, finite_bits(m[i]));
-      rmax = max(rmax, finite_bits(r[i]));
-    }
+    vmin = fminf(vmin, v[i]);
   }
+  if (!EIGHT || vmin < 0x1p-96f) {  // (zeros too; 32-bit moments are bound by memory either way)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = sqrtf(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = sqrt_from_2_96(v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) raw_set(rp, i, raw_get(rp, i) * a.decay - l.lr1 * (m[i] / (r[i] * l.ic2 + a.eps)));
   raw_store(p, e0, l.n, whole, rp);
   if constexpr (EIGHT) {
+    uint32_t mmax = 0, rmax = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      mmax = max(mmax, magnitude(m[i]));
+      rmax = max(rmax, __float_as_uint(r[i]));  // (r is not negative; a NaN is larger than infinity whatever its sign)
+    }
+    if (max(mmax, rmax) >= INF_BITS) {  // the scale is that of the finite ones
+      mmax = rmax = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        mmax = max(mmax, finite_magnitude(m[i]));
+        rmax = max(rmax, finite_magnitude(r[i]));
+      }
+    }
     // scale 2^(e-7) for a largest magnitude in [2^e, 2^(e+1)); 2^-126 where that would be no normal number
     const uint32_t mf = max(block_max(mmax) >> 23, 8u), rf = max(block_max(rmax) >> 23, 8u);
     const float minv = __uint_as_float((261u - mf) << 23), rinv = __uint_as_float((261u - rf) << 23);
-    const uint32_t key = adamw_mix(l.key ^ (uint32_t)(s0 / BLOCK)), i0 = (uint32_t)s0 & (BLOCK - 1);
+    const uint32_t key = adamw_mix(l.key ^ (uint32_t)(s0 / BLOCK)) + ((uint32_t)s0 & (BLOCK - 1));
     uint32_t cm[2] = {0, 0}, cr[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t rnd = adamw_mix(key + i0 + i);
-      cm[i / 4] |= stochastic_e4m3(m[i], minv, rnd & 0xffffu) << (8 * (i % 4));
-      const uint32_t c = stochastic_e4m3(r[i], rinv, rnd >> 16);
-      cr[i / 4] |= (r[i] > 0.f ? max(c, 1u) : c) << (8 * (i % 4));
+      const uint32_t random = adamw_mix(key + i);  // 16 bits for each of the two
+      cm[i / 4] = stochastic_e4m3(m[i] * minv, random << 16, cm[i / 4], i % 4);
+      const float q = r[i] * rinv;
+      cr[i / 4] = stochastic_e4m3(r[i] > 0.f ? fmaxf(q, 0x1p-9f) : q, random & 0xffff0000u, cr[i / 4], i % 4);  // (2^-9: the smallest value)
     }
     *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + s0) = make_uint2(cm[0], cm[1]);
     *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + s0) = make_uint2(cr[0], cr[1]);

@@ -149,8 +149,11 @@ class _Group:
         finite = bits < 0x7F800000
         field = (torch.where(finite, bits, 0).amax(1) >> 23).clamp_(min=8)
         a = x.abs() * ((261 - field) << 23).view(torch.float32)[:, None]
+        # 16 random bits are added right below the three mantissa bits that stay, and what is below those is cut.  Under 2^-6 the grid is
+        # 2^-9; one binade up a float has that grid, so 2^-6 is added there (to a multiple of 2^-29: what the sum would round is cut)
         low = a < 2.0 ** -6
-        c = ((torch.where(low, a + 2.0 ** -6, a).view(torch.int32) + (rnd << 4)) >> 20) - torch.where(low, 968, 960)
+        up = torch.floor(a * 2.0 ** 29) * 2.0 ** -29 + 2.0 ** -6
+        c = ((torch.where(low, up, a).view(torch.int32) + (rnd << 4)) >> 20) - torch.where(low, 968, 960)
         if keep_positive:
             c = torch.where(x > 0, c.clamp(min=1), c)
         c = torch.where(finite, c, 0x7F) | torch.where(torch.signbit(x), 0x80, 0)
