@@ -23,60 +23,59 @@ template <int XT> struct XType { using T = float; static constexpr int P = 3; };
 template <> struct XType<X_BF16> { using T = uint16_t; static constexpr int P = 1; };
 template <> struct XType<X_E4M3> { using T = uint8_t; static constexpr int P = 1; };
 
+__device__ __forceinline__ uint32_t word_of(float e) { return __float_as_uint(e); }
+__device__ __forceinline__ uint32_t word_of(uint16_t e) { return e; }
+__device__ __forceinline__ uint32_t word_of(uint8_t e) { return e; }
 // eight consecutive k of a row as loaded
-template <int XT> struct XRaw { typename XType<XT>::T e[8]; };
-template <int XT, bool VEC> __device__ __forceinline__ XRaw<XT> x_load(const typename XType<XT>::T* row, int k, int K) {
+template <int XT> struct XRaw { uint32_t w[2 * sizeof(typename XType<XT>::T)]; };
+template <int XT> __device__ __forceinline__ XRaw<XT> x_load(const typename XType<XT>::T* p) {
   XRaw<XT> r;
-  if constexpr (VEC) {  // (K % 8 == 0: eight of a kind.  Behind the end: the row's first eight, cleared by x_clear)
-    const auto* p = row + (k < K ? k : 0);
-    if constexpr (sizeof(r) == 8) *reinterpret_cast<uint2*>(&r) = *reinterpret_cast<const uint2*>(p);
-    else
+  __builtin_memcpy(&r, p, sizeof(r));  // (wide loads also where a row starts at an odd element)
+  return r;
+}
+// the same where the row ends among or before them: zeros from there on, nothing behind the row is read
+template <int XT> __device__ __forceinline__ XRaw<XT> x_load_end(const typename XType<XT>::T* row, int k, int K) {
+  using T = typename XType<XT>::T;
+  constexpr int PER = 4 / sizeof(T);  // elements a word
+  XRaw<XT> r;
 #pragma unroll
-      for (int i = 0; i < (int)(sizeof(r) / 16); ++i) reinterpret_cast<uint4*>(&r)[i] = reinterpret_cast<const uint4*>(p)[i];
-  } else {
+  for (int i = 0; i < (int)(2 * sizeof(T)); ++i) {
+    r.w[i] = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r.e[i] = row[min(k + i, K - 1)];
+    for (int h = 0; h < PER; ++h) {
+      const int at = k + i * PER + h;
+      const T e = row[min(at, K - 1)];
+      r.w[i] |= at < K ? word_of(e) << (8 * (int)sizeof(T) * h) : 0u;
+    }
   }
   return r;
 }
-// as bf16, with zeros behind the row's end; fp32: the part of x that column `plane` of the three takes
-template <int XT, bool VEC> __device__ __forceinline__ bf16x8 x_bf16(const XRaw<XT>& r, int k, int K, int plane) {
+// as bf16; fp32: the part of x that column `plane` of the three takes
+template <int XT> __device__ __forceinline__ bf16x8 x_bf16(const XRaw<XT>& r, int plane) {
   uint32_t u[4];
   if constexpr (XT == X_BF16) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = reinterpret_cast<const uint32_t*>(&r)[i];
+    for (int i = 0; i < 4; ++i) u[i] = r.w[i];
   } else if constexpr (XT == X_E4M3) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint32_t w = reinterpret_cast<const uint32_t*>(&r)[i];
-      u[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
-      u[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true));
+      u[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.w[i], 1.f, false));
+      u[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.w[i], 1.f, true));
     }
   } else {
+    // the upper 16 bits are taken off as often as the plane's number says (masks instead of branches: the planes are a wave's lanes).
+    // Both differences are exact.  Column 0 takes a NaN or an infinity as it is (the difference with 0 makes a NaN quiet, so that one
+    // whose bits all lie in the lower half survives); infinity less itself, a NaN, is none of the others' business.
+    const uint32_t once = plane >= 1 ? 0xffff0000u : 0u, twice = plane >= 2 ? 0xffff0000u : 0u;
+    float part[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t part[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float x = r.e[2 * i + h];
-        const uint32_t b = __float_as_uint(x), top = b & 0xffff0000u;
-        const float rest = x - __uint_as_float(top);                    // exact: the low 16 bits of the mantissa
-        const uint32_t mid = __float_as_uint(rest) & 0xffff0000u;
-        const float low = rest - __uint_as_float(mid);
-        const bool finite = (b & 0x7f800000u) != 0x7f800000u;           // an infinity goes into the first column alone
-        // (a NaN whose bits all lie in the part that is cut off stays one)
-        part[h] = plane == 0 ? (finite || (b & 0x7fffffffu) == 0x7f800000u ? top : top | 0x00400000u)
-                             : !finite ? 0u : plane == 1 ? mid : __float_as_uint(low);
-      }
-      u[i] = (part[0] >> 16) | (part[1] & 0xffff0000u);
+    for (int i = 0; i < 8; ++i) {
+      const float x = __uint_as_float(r.w[i]), y = x - __uint_as_float(r.w[i] & once);
+      part[i] = y - __uint_as_float(__float_as_uint(y) & twice);
+      part[i] = plane >= 1 && part[i] != part[i] ? 0.f : part[i];
     }
-  }
-  if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = k < K ? u[i] : 0u;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = (k + 2 * i < K ? u[i] & 0xffffu : 0u) | (k + 2 * i + 1 < K ? u[i] & 0xffff0000u : 0u);
+    for (int i = 0; i < 4; ++i) u[i] = (__float_as_uint(part[2 * i]) >> 16) | (__float_as_uint(part[2 * i + 1]) & 0xffff0000u);
   }
   return __builtin_bit_cast(bf16x8, make_uint4(u[0], u[1], u[2], u[3]));
 }
@@ -88,7 +87,7 @@ __device__ __forceinline__ bf16x8 e2m1_bf16(uint32_t w) {  // eight codes, the l
 }
 
 // GJ: matrix instructions (32 k each) that share a scale; R: tiles of 16 outputs a wave; C: tiles of 16 columns of B a wave
-template <int XT, bool VEC, int GJ, int R, int C> __global__ __launch_bounds__(1024) void linear_w4_kernel(const LinearW4Args a) {
+template <int XT, int GJ, int R, int C> __global__ __launch_bounds__(512) void linear_w4_kernel(const LinearW4Args a) {
   using T = typename XType<XT>::T;
   constexpr int P = XType<XT>::P, MC = C * 16 / P, NG = 4 / GJ;
   extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][R][16 n][C * 16 columns]
@@ -116,44 +115,69 @@ template <int XT, bool VEC, int GJ, int R, int C> __global__ __launch_bounds__(1
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[r][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int kt = wave; kt < kt_all; kt += waves) {
+  struct Weights {
     uint4 w[R];
     uint2 s[R][NG];
-    XRaw<XT> x[C][4];
+  };
+  auto load = [&](Weights& t, int kt) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      w[r] = wq[r][(long)kt * 64];
+      t.w[r] = wq[r][(long)kt * 64];
 #pragma unroll
-      for (int g = 0; g < NG; ++g) s[r][g] = *reinterpret_cast<const uint2*>(sc[r] + ((long)kt * NG + g) * 16);
+      for (int g = 0; g < NG; ++g) t.s[r][g] = *reinterpret_cast<const uint2*>(sc[r] + ((long)kt * NG + g) * 16);
     }
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[c][j] = x_load<XT, VEC>(rows[c], kt * 128 + 32 * j + 8 * kb, a.K);
+  };
+  auto multiply = [&](const Weights& t, const XRaw<XT> (&x)[C][4]) {
     bf16x8 b[C][4];
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b[c][j] = x_bf16<XT, VEC>(x[c][j], kt * 128 + 32 * j + 8 * kb, a.K, plane[c]);
+      for (int j = 0; j < 4; ++j) b[c][j] = x_bf16<XT>(x[c][j], plane[c]);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        f32x4 t[C];
+        f32x4 d[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) t[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < C; ++c) d[c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = g * GJ; j < (g + 1) * GJ; ++j) {
-          const bf16x8 wa = e2m1_bf16(reinterpret_cast<const uint32_t*>(&w[r])[j]);
+          const bf16x8 wa = e2m1_bf16(reinterpret_cast<const uint32_t*>(&t.w[r])[j]);
 #pragma unroll
-          for (int c = 0; c < C; ++c) t[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wa, b[c][j], t[c], 0, 0, 0);
+          for (int c = 0; c < C; ++c) d[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wa, b[c][j], d[c], 0, 0, 0);
         }
-        const float s4[4] = {bf2f(s[r][g].x & 0xffffu), bf2f(s[r][g].x >> 16), bf2f(s[r][g].y & 0xffffu), bf2f(s[r][g].y >> 16)};
+        const uint2 q = t.s[r][g];
+        const float s4[4] = {__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u), __uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u)};
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[r][c][i] = fmaf(t[c][i], s4[i], acc[r][c][i]);
+          for (int i = 0; i < 4; ++i) acc[r][c][i] = fmaf(d[c][i], s4[i], acc[r][c][i]);
       }
+  };
+  // Whole tiles of k.  All loads of a tile are on their way before the first is waited for (left to itself the compiler puts each load of x
+  // next to its use, a round trip to the caches each: 17 us instead of 9.5 for one row of 16384 by 2048 outputs).  Two tiles at a time
+  // gained nothing further: eight to sixteen waves a CU hide the rest.
+  const int whole = a.K / 128;
+  for (int kt = wave; kt < whole; kt += waves) {
+    Weights t;
+    XRaw<XT> x[C][4];
+    load(t, kt);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[c][j] = x_load<XT>(rows[c] + kt * 128 + 32 * j + 8 * kb);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(t, x);
+  }
+  if (whole < kt_all && wave == whole % waves) {  // the rest of k
+    Weights t;
+    XRaw<XT> x[C][4];
+    load(t, whole);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[c][j] = x_load_end<XT>(rows[c], whole * 128 + 32 * j + 8 * kb, a.K);
+    multiply(t, x);
   }
 #pragma unroll
   for (int r = 0; r < R; ++r)
@@ -180,33 +204,33 @@ template <int XT, bool VEC, int GJ, int R, int C> __global__ __launch_bounds__(1
 }
 
 namespace {
-template <int XT, bool VEC, int GJ, int R, int C> void go(const LinearW4Args& a, int waves, hipStream_t st) {
+template <int XT, int GJ, int R, int C> void go(const LinearW4Args& a, hipStream_t st) {
   constexpr int MC = C * 16 / XType<XT>::P;
-  const int nt = (a.N + 15) / 16;
-  hipLaunchKernelGGL((linear_w4_kernel<XT, VEC, GJ, R, C>), dim3((nt + R - 1) / R, (unsigned)((a.M + MC - 1) / MC)), dim3(64 * waves),
+  // eight waves split k (16 were as fast at best; 4 took 9 instead of 7 us where 65 workgroups share 25 tiles of k, and are even elsewhere)
+  const int nt = (a.N + 15) / 16, kt = (a.K + 127) / 128, waves = kt < 8 ? kt : 8;
+  hipLaunchKernelGGL((linear_w4_kernel<XT, GJ, R, C>), dim3((nt + R - 1) / R, (unsigned)((a.M + MC - 1) / MC)), dim3(64 * waves),
                      sizeof(float) * waves * R * 256 * C, st, a);
 }
-template <int XT, bool VEC, int GJ> void with_tiles(const LinearW4Args& a, hipStream_t st) {
+// Rows whose columns fit one tile of B: the more tiles of outputs a wave takes, the less often x is read and converted (from the
+// caches, but 16 rows of bf16 are four times a tile's weights), as long as the workgroups still fill the chip.  Measured, us with 1 / 2 / 4
+// tiles: 4096 outputs (16 rows bf16, k 4096) 6.9 / 8.2 / -; 8192 (1 row bf16, k 8192) 10.4 / 8.2 / 11.0; 16384 (16 rows e4m3, k 16384)
+// 68 / 42 / 32.  fp32 rows hold three times the registers: two tiles of outputs or of columns at most (4: 19.8 instead of 15.4 us for
+// 5 rows, 8192 x 8192).
+template <int XT, int GJ> void with_tiles(const LinearW4Args& a, hipStream_t st) {
   const long cols = a.M * XType<XT>::P;
-  const int nt = (a.N + 15) / 16, kt = (a.K + 127) / 128;
-  // waves of a workgroup: as many as there are k tiles, up to 16; 8 where the outputs alone fill the chip (256 CUs of 32 waves)
-  const int most = nt >= 512 ? 8 : 16, waves = kt < most ? kt : most;
-  // (fp32 rows hold more registers: at most two tiles of columns, one where elements are loaded one by one)
-  if constexpr (XT != X_F32)
-    if (cols > 32) return go<XT, VEC, GJ, 1, 4>(a, waves < 8 ? waves : 8, st);
-  if constexpr (XT != X_F32 || VEC)
-    if (cols > 16) return go<XT, VEC, GJ, 1, 2>(a, waves < 8 ? waves : 8, st);
-  go<XT, VEC, GJ, 1, 1>(a, waves, st);
+  const int nt = (a.N + 15) / 16;
+  if constexpr (XT != X_F32) {
+    if (cols > 32) return go<XT, GJ, 1, 4>(a, st);
+    if (cols <= 16 && nt >= 1024) return go<XT, GJ, 4, 1>(a, st);
+  }
+  if (cols > 16) return go<XT, GJ, 1, 2>(a, st);
+  if (nt >= 512) return go<XT, GJ, 2, 1>(a, st);
+  go<XT, GJ, 1, 1>(a, st);
 }
-template <int XT, bool VEC> void with_group(const LinearW4Args& a, hipStream_t st) {
-  if (a.group == 32) with_tiles<XT, VEC, 1>(a, st);
-  else if (a.group == 64) with_tiles<XT, VEC, 2>(a, st);
-  else with_tiles<XT, VEC, 4>(a, st);
-}
-template <int XT> void with_rows(const LinearW4Args& a, hipStream_t st) {
-  constexpr int size = (int)sizeof(typename XType<XT>::T), piece = 8 * size < 16 ? 8 * size : 16;  // bytes of one load
-  if (a.K % 8 == 0 && (uintptr_t)a.x % piece == 0 && a.ldx * size % piece == 0) with_group<XT, true>(a, st);
-  else with_group<XT, false>(a, st);
+template <int XT> void with_group(const LinearW4Args& a, hipStream_t st) {
+  if (a.group == 32) with_tiles<XT, 1>(a, st);
+  else if (a.group == 64) with_tiles<XT, 2>(a, st);
+  else with_tiles<XT, 4>(a, st);
 }
 }  // namespace
 
@@ -214,9 +238,9 @@ DTF_API int dtf_linear_w4(const LinearW4Args* p, hipStream_t st) {
   if (!p || !p->x || !p->wq || !p->scales || !p->y || p->M <= 0 || p->N <= 0 || p->K <= 0 || p->ldx < 0) return ERR;
   if ((p->group != 32 && p->group != 64 && p->group != 128) || p->xtype < 0 || p->xtype > 2) return ERR;
   if ((uintptr_t)p->wq % 16 || (uintptr_t)p->scales % 8 || p->M > 65535L * 5) return ERR;  // (grid.y: five rows and more each)
-  if (p->xtype == X_F32) with_rows<X_F32>(*p, st);
-  else if (p->xtype == X_BF16) with_rows<X_BF16>(*p, st);
-  else with_rows<X_E4M3>(*p, st);
+  if (p->xtype == X_F32) with_group<X_F32>(*p, st);
+  else if (p->xtype == X_BF16) with_group<X_BF16>(*p, st);
+  else with_group<X_E4M3>(*p, st);
   DTF_CHECK_LAUNCH();
   return 0;
 }
