@@ -86,22 +86,15 @@ __device__ __forceinline__ bf16x8 e2m1_bf16(uint32_t w) {  // eight codes, the l
                                                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 3))));
 }
 
-// GJ: matrix instructions (32 k each) that share a scale; R: tiles of 16 outputs a wave; C: tiles of 16 columns of B a wave
-template <int XT, int GJ, int R, int C> __global__ __launch_bounds__(512) void linear_w4_kernel(const LinearW4Args a) {
+// GJ: matrix instructions (32 k each) that share a scale; R: tiles of 16 outputs a wave
+template <int XT, int GJ, int R> __global__ __launch_bounds__(512) void linear_w4_kernel(const LinearW4Args a) {
   using T = typename XType<XT>::T;
-  constexpr int P = XType<XT>::P, MC = C * 16 / P, NG = 4 / GJ;
-  extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][R][16 n][C * 16 columns]
+  constexpr int P = XType<XT>::P, MC = 16 / P, NG = 4 / GJ;
+  extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][R][16 n][16 columns]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, kb = lane >> 4, col = lane & 15;
-  const int nt_all = (a.N + 15) / 16, kt_all = (a.K + 127) / 128, nt0 = blockIdx.x * R;
-  const long m0 = (long)blockIdx.y * MC;
-  const T* rows[C];
-  int plane[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {  // (columns behind the last row repeat it: nothing of theirs is stored)
-    const long m = m0 + (16 * c + col) / P;
-    rows[c] = static_cast<const T*>(a.x) + (m < a.M ? m : a.M - 1) * a.ldx;
-    plane[c] = (16 * c + col) % P;
-  }
+  const int nt_all = (a.N + 15) / 16, kt_all = (a.K + 127) / 128, nt0 = blockIdx.x * R, plane = col % P;
+  const long m0 = (long)blockIdx.y * MC, mine = min(m0 + col / P, a.M - 1);  // (columns behind the last row repeat it: not stored)
+  const T* row = static_cast<const T*>(a.x) + mine * a.ldx;
   const uint4* wq[R];
   const uint16_t* sc[R];
 #pragma unroll
@@ -110,11 +103,9 @@ template <int XT, int GJ, int R, int C> __global__ __launch_bounds__(512) void l
     wq[r] = static_cast<const uint4*>(a.wq) + nt * kt_all * 64 + lane;
     sc[r] = a.scales + nt * kt_all * NG * 16 + 4 * kb;
   }
-  f32x4 acc[R][C];
+  f32x4 acc[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int c = 0; c < C; ++c) acc[r][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int r = 0; r < R; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
   struct Weights {
     uint4 w[R];
     uint2 s[R][NG];
@@ -127,31 +118,22 @@ template <int XT, int GJ, int R, int C> __global__ __launch_bounds__(512) void l
       for (int g = 0; g < NG; ++g) t.s[r][g] = *reinterpret_cast<const uint2*>(sc[r] + ((long)kt * NG + g) * 16);
     }
   };
-  auto multiply = [&](const Weights& t, const XRaw<XT> (&x)[C][4]) {
-    bf16x8 b[C][4];
+  auto multiply = [&](const Weights& t, const XRaw<XT> (&x)[4]) {
+    bf16x8 b[4];
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b[c][j] = x_bf16<XT>(x[c][j], plane[c]);
+    for (int j = 0; j < 4; ++j) b[j] = x_bf16<XT>(x[j], plane);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        f32x4 d[C];
+        f32x4 d = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < C; ++c) d[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = g * GJ; j < (g + 1) * GJ; ++j) {
-          const bf16x8 wa = e2m1_bf16(reinterpret_cast<const uint32_t*>(&t.w[r])[j]);
-#pragma unroll
-          for (int c = 0; c < C; ++c) d[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wa, b[c][j], d[c], 0, 0, 0);
-        }
+        for (int j = g * GJ; j < (g + 1) * GJ; ++j)
+          d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e2m1_bf16(reinterpret_cast<const uint32_t*>(&t.w[r])[j]), b[j], d, 0, 0, 0);
         const uint2 q = t.s[r][g];
         const float s4[4] = {__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u), __uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u)};
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[r][c][i] = fmaf(d[c][i], s4[i], acc[r][c][i]);
+        for (int i = 0; i < 4; ++i) acc[r][i] = fmaf(d[i], s4[i], acc[r][i]);
       }
   };
   // Whole tiles of k.  All loads of a tile are on their way before the first is waited for (left to itself the compiler puts each load of x
@@ -160,31 +142,25 @@ template <int XT, int GJ, int R, int C> __global__ __launch_bounds__(512) void l
   const int whole = a.K / 128;
   for (int kt = wave; kt < whole; kt += waves) {
     Weights t;
-    XRaw<XT> x[C][4];
+    XRaw<XT> x[4];
     load(t, kt);
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[c][j] = x_load<XT>(rows[c] + kt * 128 + 32 * j + 8 * kb);
+    for (int j = 0; j < 4; ++j) x[j] = x_load<XT>(row + kt * 128 + 32 * j + 8 * kb);
     __builtin_amdgcn_sched_barrier(0);
     multiply(t, x);
   }
   if (whole < kt_all && wave == whole % waves) {  // the rest of k
     Weights t;
-    XRaw<XT> x[C][4];
+    XRaw<XT> x[4];
     load(t, whole);
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[c][j] = x_load_end<XT>(rows[c], whole * 128 + 32 * j + 8 * kb, a.K);
+    for (int j = 0; j < 4; ++j) x[j] = x_load_end<XT>(row, whole * 128 + 32 * j + 8 * kb, a.K);
     multiply(t, x);
   }
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) part[((wave * R + r) * 16 + 4 * kb + i) * (C * 16) + 16 * c + col] = acc[r][c][i];
+    for (int i = 0; i < 4; ++i) part[((wave * R + r) * 16 + 4 * kb + i) * 16 + col] = acc[r][i];
   __syncthreads();
   for (int o = threadIdx.x; o < R * 16 * MC; o += blockDim.x) {
     const int n = o % (R * 16), mm = o / (R * 16);
@@ -194,7 +170,7 @@ template <int XT, int GJ, int R, int C> __global__ __launch_bounds__(512) void l
     float s = 0.f;
     for (int w = 0; w < waves; ++w)
 #pragma unroll
-      for (int p = 0; p < P; ++p) s += part[(w * R * 16 + n) * (C * 16) + mm * P + p];
+      for (int p = 0; p < P; ++p) s += part[(w * R * 16 + n) * 16 + mm * P + p];
     if (a.x_scale) s *= a.x_scale[m];
     if (a.bias) s += a.bias[out];
     if (a.relu) s = s < 0.f ? 0.f : s;  // (a NaN stays one)
@@ -204,28 +180,23 @@ template <int XT, int GJ, int R, int C> __global__ __launch_bounds__(512) void l
 }
 
 namespace {
-template <int XT, int GJ, int R, int C> void go(const LinearW4Args& a, hipStream_t st) {
-  constexpr int MC = C * 16 / XType<XT>::P;
+template <int XT, int GJ, int R> void go(const LinearW4Args& a, int passes, hipStream_t st) {
   // eight waves split k (16 were as fast at best; 4 took 9 instead of 7 us where 65 workgroups share 25 tiles of k, and are even elsewhere)
   const int nt = (a.N + 15) / 16, kt = (a.K + 127) / 128, waves = kt < 8 ? kt : 8;
-  hipLaunchKernelGGL((linear_w4_kernel<XT, GJ, R, C>), dim3((nt + R - 1) / R, (unsigned)((a.M + MC - 1) / MC)), dim3(64 * waves),
-                     sizeof(float) * waves * R * 256 * C, st, a);
+  hipLaunchKernelGGL((linear_w4_kernel<XT, GJ, R>), dim3((nt + R - 1) / R, passes), dim3(64 * waves), sizeof(float) * waves * R * 256, st, a);
 }
-// Rows whose columns fit one tile of B: the more tiles of outputs a wave takes, the less often x is read and converted (from the
-// caches, but 16 rows of bf16 are four times a tile's weights), as long as the workgroups still fill the chip.  Measured, us with 1 / 2 / 4
-// tiles: 4096 outputs (16 rows bf16, k 4096) 6.9 / 8.2 / -; 8192 (1 row bf16, k 8192) 10.4 / 8.2 / 11.0; 16384 (16 rows e4m3, k 16384)
-// 68 / 42 / 32.  fp32 rows hold three times the registers: two tiles of outputs or of columns at most (4: 19.8 instead of 15.4 us for
-// 5 rows, 8192 x 8192).
+// More rows than the columns of B hold (16; fp32 5) take a pass over the weights for each such set, side by side in one launch: several
+// column tiles a wave were slower, because x is what a wave reads most (16 rows of bf16 are four times a tile's weights): 64 rows of bf16,
+// 4096 x 16384: 30.6 us, with four column tiles a wave 35.5.  For the same reason the tiles of outputs a wave takes are as many as leave
+// the chip filled.  Measured, us with 1 / 2 / 4 tiles, by tiles of outputs x passes (k 4096): 256 (2048 outputs, 32 rows bf16) 6.8 / 8.2 / 10.5;
+// 512 (8192, 16 rows bf16) 11.2 / 8.6 / 10.7; 1024 (16384, 16 rows bf16) 19.5 / 13.4 / 11.3, (16384, 5 rows fp32) 20.2 / 14.1 / 13.0.
 template <int XT, int GJ> void with_tiles(const LinearW4Args& a, hipStream_t st) {
-  const long cols = a.M * XType<XT>::P;
-  const int nt = (a.N + 15) / 16;
-  if constexpr (XT != X_F32) {
-    if (cols > 32) return go<XT, GJ, 1, 4>(a, st);
-    if (cols <= 16 && nt >= 1024) return go<XT, GJ, 4, 1>(a, st);
-  }
-  if (cols > 16) return go<XT, GJ, 1, 2>(a, st);
-  if (nt >= 512) return go<XT, GJ, 2, 1>(a, st);
-  go<XT, GJ, 1, 1>(a, st);
+  constexpr int MC = 16 / XType<XT>::P;
+  const int passes = (int)((a.M + MC - 1) / MC);
+  const long sets = (long)((a.N + 15) / 16) * passes;
+  if (sets >= 1024) go<XT, GJ, 4>(a, passes, st);
+  else if (sets >= 512) go<XT, GJ, 2>(a, passes, st);
+  else go<XT, GJ, 1>(a, passes, st);
 }
 template <int XT> void with_group(const LinearW4Args& a, hipStream_t st) {
   if (a.group == 32) with_tiles<XT, 1>(a, st);
