@@ -17,7 +17,7 @@ struct RmsNormArgs {
   long rows, ld_x, ld_res, ld_dy, ld_dh;
   int dim, bf16;
   float eps;
-  int blocks;         // backward: rows of `part`
+  int blocks;         // backward: rows of `part` (dtf_rms_norm_bwd_blocks; 0: no `part`)
 };
 
 extern "C" int dtf_rms_norm_fwd(const RmsNormArgs* a, hipStream_t st);

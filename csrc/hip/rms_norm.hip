@@ -10,6 +10,7 @@
 // those in a fixed order (no atomics: the same result on every run).
 #include "common.h"
 #include "rms_norm.h"
+#include <type_traits>
 
 namespace {
 constexpr int ERR = -22;
@@ -198,12 +199,36 @@ __global__ __launch_bounds__(1024) void rms_norm_fwd_long_kernel(const RmsNormAr
   }
 }
 
+// 16 columns of dw from all rows: 256 threads = 16 columns x 16 sets of rows, then the sets' sums in order
+template <typename T, bool RES> __device__ __forceinline__ void dw_columns(const RmsNormArgs& a, int c0, float (*sums)[17]) {
+  const int c = c0 + (threadIdx.x & 15), set = threadIdx.x >> 4, cc = min(c, a.dim - 1);
+  float s = 0.f;
+#pragma unroll 8
+  for (long row = set; row < a.rows; row += 16) {
+    float h = load_piece<T, 1>(static_cast<const T*>(a.x) + row * a.ld_x + cc).get(0);
+    if constexpr (RES) h += load_piece<T, 1>(static_cast<const T*>(a.res) + row * a.ld_res + cc).get(0);
+    s += load_piece<T, 1>(static_cast<const T*>(a.dy) + row * a.ld_dy + cc).get(0) * (h * a.rstd[row]);
+  }
+  sums[set][threadIdx.x & 15] = s;
+  __syncthreads();
+  if (set || c >= a.dim) return;
+  for (int i = 1; i < 16; ++i) s += sums[i][threadIdx.x & 15];
+  a.dw[c] = s;
+}
+
 // Every workgroup takes rows blockIdx, blockIdx + gridDim, ... (four at a time with a wave a row); w and the sums of dw stay in registers.
-template <typename T, int VEC, int NT, int IT, bool RES, bool DH>
+// SPLIT, for few rows: dw does not wait for the rows' sums, so that further workgroups of the same launch take it, 16 columns each, and
+// no partial sums go through memory.
+template <typename T, int VEC, int NT, int IT, bool RES, bool DH, bool SPLIT>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rms_norm_bwd_kernel(const RmsNormArgs a) {
   constexpr int RPB = NT < 256 ? 256 / NT : 1;
   __shared__ float slots[2][NT < 256 ? 1 : NT / 64];
   __shared__ __attribute__((aligned(16))) float sums[NT < 256 ? IT * NT * VEC : 1];
+  if constexpr (SPLIT) {
+    __shared__ float sets[16][17];
+    const int rows_wg = (int)((a.rows + RPB - 1) / RPB);
+    if ((int)blockIdx.x >= rows_wg) return dw_columns<T, RES>(a, ((int)blockIdx.x - rows_wg) * 16, sets);
+  }
   const int t = threadIdx.x % NT, group = threadIdx.x / NT, pieces = a.dim / VEC;
   const float over = 1.f / (float)a.dim;
   float w[IT][VEC], acc[IT][VEC];
@@ -214,7 +239,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rms_norm_bwd_kernel(const
     for (int i = 0; i < VEC; ++i) acc[k][i] = 0.f;
   }
   int parity = 0;
-  for (long row = (long)blockIdx.x * RPB + group; row < a.rows; row += (long)gridDim.x * RPB) {
+  for (long row = (long)blockIdx.x * RPB + group; row < a.rows; row += SPLIT ? a.rows : (long)gridDim.x * RPB) {
     const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
     const T* res = static_cast<const T*>(a.res) + row * a.ld_res;
     const T* dy = static_cast<const T*>(a.dy) + row * a.ld_dy;
@@ -239,7 +264,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rms_norm_bwd_kernel(const
         n[k][i] = px[k].get(i);
         if constexpr (RES) n[k][i] += pr[k].get(i);
         n[k][i] *= rstd;
-        acc[k][i] += d * n[k][i];
+        if constexpr (!SPLIT) acc[k][i] += d * n[k][i];
         dot += in ? d * w[k][i] * n[k][i] : 0.f;
       }
     }
@@ -258,7 +283,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rms_norm_bwd_kernel(const
       store_piece<T, VEC>(static_cast<T*>(a.y) + row * a.dim + (k * NT + t) * VEC, p);
     }
   }
-  if (!a.part) return;
+  if (SPLIT || !a.part) return;
   if constexpr (NT < 256) {  // the four waves' sums, in the waves' order
     for (int g = 0; g < RPB; ++g) {
       if (group == g)
@@ -406,25 +431,37 @@ DTF_API int dtf_rms_norm_fwd(const RmsNormArgs* p, hipStream_t st) {
   return 0;
 }
 
-// How many rows of partial sums `part` the backward pass of these sizes writes.
+// How many rows of partial sums `part` the backward pass of these sizes writes; 0: none (dw in the same launch as dx).
+// One launch / two, us: 100 x 1024 fp32 2.5 / 6.0, 512 x 1024 fp32 3.3 / 6.6, 512 x 2048 bf16 3.5 / 8.1, 1000 x 2048 bf16 9.5 / 9.0 (x and dy
+// are read twice, and a thread takes a sixteenth of the rows).
 DTF_API int dtf_rms_norm_bwd_blocks(long rows, int dim) {
   if (rows <= 0 || dim <= 0) return ERR;
+  if (rows <= 512 && dim <= 4096) return 0;
   return (int)(rows < 512 ? rows : 512);
 }
 
 DTF_API int dtf_rms_norm_bwd(const RmsNormArgs* p, hipStream_t st) {
-  if (bad(p) || !p->dy || !p->rstd || (p->dw && !p->part) || p->blocks != dtf_rms_norm_bwd_blocks(p->rows, p->dim)) return ERR;
+  if (bad(p) || !p->dy || !p->rstd || p->blocks != dtf_rms_norm_bwd_blocks(p->rows, p->dim) || (p->dw && p->blocks && !p->part)) return ERR;
   const RmsNormArgs a = *p;
   const bool done = with_vec(a, aligned(a), few_rows(a), [&](auto type, auto s) {
     using T = decltype(type);
     using S = decltype(s);
-    const dim3 grid(a.blocks), block(S::NT < 256 ? 256 : S::NT);
+    const dim3 block(S::NT < 256 ? 256 : S::NT);
+    auto go = [&](auto res, auto dh) {
+      constexpr bool RES = decltype(res)::value, DH = decltype(dh)::value;
+      if constexpr (S::NT <= 256)
+        if (a.blocks == 0) {
+          const long rows_wg = S::NT < 256 ? (a.rows + 256 / S::NT - 1) / (256 / S::NT) : a.rows;
+          hipLaunchKernelGGL((rms_norm_bwd_kernel<T, S::VEC, S::NT, S::IT, RES, DH, true>), dim3((unsigned)rows_wg + (a.dw ? (a.dim + 15) / 16 : 0)),
+                             block, 0, st, a);
+          return;
+        }
+      hipLaunchKernelGGL((rms_norm_bwd_kernel<T, S::VEC, S::NT, S::IT, RES, DH, false>), dim3(a.blocks), block, 0, st, a);
+    };
     if (a.res) {
-      if (a.dh) hipLaunchKernelGGL((rms_norm_bwd_kernel<T, S::VEC, S::NT, S::IT, true, true>), grid, block, 0, st, a);
-      else hipLaunchKernelGGL((rms_norm_bwd_kernel<T, S::VEC, S::NT, S::IT, true, false>), grid, block, 0, st, a);
+      if (a.dh) go(std::true_type{}, std::true_type{}); else go(std::true_type{}, std::false_type{});
     } else {
-      if (a.dh) hipLaunchKernelGGL((rms_norm_bwd_kernel<T, S::VEC, S::NT, S::IT, false, true>), grid, block, 0, st, a);
-      else hipLaunchKernelGGL((rms_norm_bwd_kernel<T, S::VEC, S::NT, S::IT, false, false>), grid, block, 0, st, a);
+      if (a.dh) go(std::false_type{}, std::true_type{}); else go(std::false_type{}, std::false_type{});
     }
   });
   if (!done) {
@@ -436,7 +473,7 @@ DTF_API int dtf_rms_norm_bwd(const RmsNormArgs* p, hipStream_t st) {
     if (a.bf16) go(uint16_t{}); else go(float{});
   }
   DTF_CHECK_LAUNCH();
-  if (a.dw) hipLaunchKernelGGL(rms_norm_dw_kernel, dim3(dtf_cdiv(a.dim, 64)), dim3(1024), 0, st, a.part, a.dw, a.blocks, a.dim);
+  if (a.dw && a.blocks) hipLaunchKernelGGL(rms_norm_dw_kernel, dim3(dtf_cdiv(a.dim, 64)), dim3(1024), 0, st, a.part, a.dw, a.blocks, a.dim);
   DTF_CHECK_LAUNCH();
   return 0;
 }

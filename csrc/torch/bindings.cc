@@ -126,9 +126,11 @@ std::tuple<Tensor, OptTensor> rms_norm_backward(const Tensor& dy, const Tensor& 
   Tensor part;
   if (need_dw) {
     dw = at::empty(w.sizes(), w.options());
-    part = at::empty({a.blocks, a.dim}, w.options());
     a.dw = dw->mutable_data_ptr<float>();
-    a.part = part.mutable_data_ptr<float>();
+    if (a.blocks) {
+      part = at::empty({a.blocks, a.dim}, w.options());
+      a.part = part.mutable_data_ptr<float>();
+    }
   }
   if (rr) {
     a.res = rr->p;

@@ -36,7 +36,8 @@ def check_e4m3(q, scale, x, w, res, eps):
 def check_backward(dx, dw, dy, x, rstd, w, res, dh):
     """From rstd as it was saved.  Every term of mean(g h rstd) carries 4 roundings and those of its sums (below 48): 64 U of the
     mean of magnitudes, on top of a few for the rest: dx within 64 U of the magnitudes of its terms, and its type's rounding.
-    dw: terms of 3 roundings, and the sums over rows (a workgroup's rows / 512, four waves, 512 / 16 rows of partial sums, 16 waves)."""
+    dw: terms of 3 roundings, and the sums over rows (a workgroup's rows / 512, four waves, 512 / 16 rows of partial sums, 16 waves; up to 512 rows
+    a thread's rows / 16 and 16 sets: 48)."""
     h64, dy64, w64, rstd = x.double() + (0.0 if res is None else res.double()), dy.double(), w.double(), rstd.double()[..., None]
     dim, d = x.shape[-1], x.dtype
     n, g = h64 * rstd, dy64 * w64

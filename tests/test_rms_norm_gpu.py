@@ -8,7 +8,8 @@ pytestmark = pytest.mark.gpu
 F, B = torch.float32, torch.bfloat16
 # (rows, dim): one element; a wave a row with 1, 2, 4 pieces; odd widths; 256 and 1024 threads; rows longer than a workgroup's registers
 SHAPES = [(1, 1), (3, 7), (1, 2048), (5, 256), (1500, 512), (1030, 1024), (1027, 2048), (33, 1000), (6, 1001), (2, 3137), (700, 4096), (4, 4100),
-          (3, 8192), (2, 8199), (2, 16384), (2, 20000), (1025, 129), (1100, 250)]
+          (3, 8192), (2, 8199), (2, 16384), (2, 20000), (1025, 129), (1100, 250), (512, 2048), (513, 2048),
+          (511, 1000), (300, 4097)]
 
 
 def _rand(gen, *shape, dtype=F):
