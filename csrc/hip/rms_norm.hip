@@ -29,22 +29,21 @@ template <typename T, int VEC> struct Piece {  // VEC consecutive elements as lo
     else e[i] = f2bf(v);
   }
 };
+// (wide accesses whatever the address: rows of odd lengths start anywhere)
 template <typename T, int VEC> __device__ __forceinline__ Piece<T, VEC> load_piece(const T* p) {
   Piece<T, VEC> r;
-  if constexpr (sizeof(r) == 16) *reinterpret_cast<uint4*>(&r) = *reinterpret_cast<const uint4*>(p);
-  else r.e[0] = *p;
+  __builtin_memcpy(&r, p, sizeof(r));
   return r;
 }
-template <typename T, int VEC> __device__ __forceinline__ void store_piece(T* p, const Piece<T, VEC>& r) {
-  if constexpr (sizeof(r) == 16) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&r);
-  else *p = r.e[0];
-}
-template <int VEC> __device__ __forceinline__ void load_w(const float* p, float* w) {
-  if constexpr (VEC == 1) w[0] = *p;
-  else
-#pragma unroll
-    for (int i = 0; i < VEC; i += 4) *reinterpret_cast<float4*>(w + i) = *reinterpret_cast<const float4*>(p + i);
-}
+template <typename T, int VEC> __device__ __forceinline__ void store_piece(T* p, const Piece<T, VEC>& r) { __builtin_memcpy(p, &r, sizeof(r)); }
+template <int VEC> __device__ __forceinline__ void load_w(const float* p, float* w) { __builtin_memcpy(w, p, VEC * sizeof(float)); }
+// Piece number c of a row: the last one ends where the row ends and covers some elements of the one before again (the same values are
+// computed and stored twice); `skip` says how many, so that sums count them once.  Numbers behind the last: that one again, all skipped.
+template <int VEC> struct Place {
+  int start, skip;
+  bool in;
+  __device__ __forceinline__ Place(int c, int dim) : start(min(c * VEC, dim - VEC)), skip(min(c * VEC - start, VEC)), in(c * VEC < dim) {}
+};
 // VEC floats as e4m3 (to nearest even)
 template <int VEC> __device__ __forceinline__ void store_e4m3(uint8_t* p, const float* y) {
   if constexpr (VEC == 1) *p = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[0], 0.f, 0, false);
@@ -55,8 +54,7 @@ template <int VEC> __device__ __forceinline__ void store_e4m3(uint8_t* p, const 
       u[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
       u[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], (int)u[i], true);
     }
-    if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(p) = u[0];
-    else *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+    __builtin_memcpy(p, u, VEC);
   }
 }
 
@@ -95,7 +93,7 @@ template <typename T, int VEC, int NT, int IT, bool RES, bool OUT8>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rms_norm_fwd_kernel(const RmsNormArgs a) {
   constexpr int RPB = NT < 256 ? 256 / NT : 1;
   __shared__ float slots[2][NT < 256 ? 1 : NT / 64];
-  const int t = threadIdx.x % NT, pieces = a.dim / VEC;
+  const int t = threadIdx.x % NT;
   const long row = (long)blockIdx.x * RPB + threadIdx.x / NT;
   if (row >= a.rows) return;  // (whole waves; a workgroup a row has none)
   const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
@@ -104,26 +102,26 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rms_norm_fwd_kernel(const
   float w[IT][VEC];
 #pragma unroll
   for (int k = 0; k < IT; ++k) {
-    const int c = min(k * NT + t, pieces - 1);  // (pieces behind the end: the last one again, not counted and not stored)
-    px[k] = load_piece<T, VEC>(x + c * VEC);
-    if constexpr (RES) pr[k] = load_piece<T, VEC>(res + c * VEC);
+    const Place<VEC> at(k * NT + t, a.dim);
+    px[k] = load_piece<T, VEC>(x + at.start);
+    if constexpr (RES) pr[k] = load_piece<T, VEC>(res + at.start);
   }
 #pragma unroll
-  for (int k = 0; k < IT; ++k) load_w<VEC>(a.w + min(k * NT + t, pieces - 1) * VEC, w[k]);
+  for (int k = 0; k < IT; ++k) load_w<VEC>(a.w + Place<VEC>(k * NT + t, a.dim).start, w[k]);
   float v[IT][VEC], ss = 0.f;
 #pragma unroll
   for (int k = 0; k < IT; ++k) {
-    const bool in = k * NT + t < pieces;
+    const Place<VEC> at(k * NT + t, a.dim);
     Piece<T, VEC> ph;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       v[k][i] = px[k].get(i);
       if constexpr (RES) v[k][i] += pr[k].get(i);
-      ss += in ? v[k][i] * v[k][i] : 0.f;
+      ss += i >= at.skip ? v[k][i] * v[k][i] : 0.f;
       ph.set(i, v[k][i]);
     }
     if constexpr (RES)
-      if (in) store_piece<T, VEC>(static_cast<T*>(a.h) + row * a.dim + (k * NT + t) * VEC, ph);
+      if (at.in) store_piece<T, VEC>(static_cast<T*>(a.h) + row * a.dim + at.start, ph);
   }
   const float rstd = 1.f / sqrtf(row_sum<NT>(ss, slots[0]) / (float)a.dim + a.eps);
   if (a.rstd && t == 0) a.rstd[row] = rstd;
@@ -142,8 +140,9 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rms_norm_fwd_kernel(const
   }
 #pragma unroll
   for (int k = 0; k < IT; ++k) {
-    if (k * NT + t >= pieces) continue;
-    const long at = row * a.dim + (k * NT + t) * VEC;
+    const Place<VEC> place(k * NT + t, a.dim);
+    if (!place.in) continue;
+    const long at = row * a.dim + place.start;
     if constexpr (OUT8) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[k][i] *= inv;
@@ -229,12 +228,12 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rms_norm_bwd_kernel(const
     const int rows_wg = (int)((a.rows + RPB - 1) / RPB);
     if ((int)blockIdx.x >= rows_wg) return dw_columns<T, RES>(a, ((int)blockIdx.x - rows_wg) * 16, sets);
   }
-  const int t = threadIdx.x % NT, group = threadIdx.x / NT, pieces = a.dim / VEC;
+  const int t = threadIdx.x % NT, group = threadIdx.x / NT;
   const float over = 1.f / (float)a.dim;
   float w[IT][VEC], acc[IT][VEC];
 #pragma unroll
   for (int k = 0; k < IT; ++k) {
-    load_w<VEC>(a.w + min(k * NT + t, pieces - 1) * VEC, w[k]);
+    load_w<VEC>(a.w + Place<VEC>(k * NT + t, a.dim).start, w[k]);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) acc[k][i] = 0.f;
   }
@@ -247,17 +246,17 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rms_norm_bwd_kernel(const
     Piece<T, VEC> px[IT], pr[IT], pd[IT], pg[IT];
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
-      const int c = min(k * NT + t, pieces - 1);
-      px[k] = load_piece<T, VEC>(x + c * VEC);
-      if constexpr (RES) pr[k] = load_piece<T, VEC>(res + c * VEC);
-      pd[k] = load_piece<T, VEC>(dy + c * VEC);
-      if constexpr (DH) pg[k] = load_piece<T, VEC>(dh + c * VEC);
+      const int start = Place<VEC>(k * NT + t, a.dim).start;
+      px[k] = load_piece<T, VEC>(x + start);
+      if constexpr (RES) pr[k] = load_piece<T, VEC>(res + start);
+      pd[k] = load_piece<T, VEC>(dy + start);
+      if constexpr (DH) pg[k] = load_piece<T, VEC>(dh + start);
     }
     const float rstd = a.rstd[row];
     float dot = 0.f, n[IT][VEC];  // n = h rstd
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
-      const bool in = k * NT + t < pieces;
+      const int skip = Place<VEC>(k * NT + t, a.dim).skip;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const float d = pd[k].get(i);
@@ -265,14 +264,15 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rms_norm_bwd_kernel(const
         if constexpr (RES) n[k][i] += pr[k].get(i);
         n[k][i] *= rstd;
         if constexpr (!SPLIT) acc[k][i] += d * n[k][i];
-        dot += in ? d * w[k][i] * n[k][i] : 0.f;
+        dot += i >= skip ? d * w[k][i] * n[k][i] : 0.f;
       }
     }
     const float mean = row_sum<NT>(dot, slots[parity]) * over;  // (two sets of slots: one barrier a row)
     parity ^= 1;
 #pragma unroll
     for (int k = 0; k < IT; ++k) {
-      if (k * NT + t >= pieces) continue;
+      const Place<VEC> at(k * NT + t, a.dim);
+      if (!at.in) continue;
       Piece<T, VEC> p;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
@@ -280,7 +280,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rms_norm_bwd_kernel(const
         if constexpr (DH) v += pg[k].get(i);
         p.set(i, v);
       }
-      store_piece<T, VEC>(static_cast<T*>(a.y) + row * a.dim + (k * NT + t) * VEC, p);
+      store_piece<T, VEC>(static_cast<T*>(a.y) + row * a.dim + at.start, p);
     }
   }
   if (SPLIT || !a.part) return;
@@ -301,12 +301,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rms_norm_bwd_kernel(const
   }
 #pragma unroll
   for (int k = 0; k < IT; ++k) {
-    if (k * NT + t >= pieces) continue;
-    float* p = a.part + (long)blockIdx.x * a.dim + (k * NT + t) * VEC;
-    if constexpr (VEC == 1) *p = acc[k][0];
-    else
-#pragma unroll
-      for (int i = 0; i < VEC; i += 4) *reinterpret_cast<float4*>(p + i) = *reinterpret_cast<const float4*>(&acc[k][i]);
+    const Place<VEC> at(k * NT + t, a.dim);
+    if (at.in) __builtin_memcpy(a.part + (long)blockIdx.x * a.dim + at.start, acc[k], VEC * sizeof(float));
   }
 }
 
@@ -359,39 +355,27 @@ __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* __restri
 namespace {
 template <int VEC_, int NT_, int IT_> struct Shape { static constexpr int VEC = VEC_, NT = NT_, IT = IT_; };
 
-// The threads of a row and the pieces of a thread, so that a thread holds at most 32 elements (16 where elements are loaded one by
-// one): a wave a row while that is enough (no barrier, four rows a workgroup), then 256 or 1024 threads.  `few`: rows that leave
-// most of the chip idle take 256 threads at once.  False: the row does not fit.
-template <int VEC, typename F> bool with_shape(int pieces, bool few, F f) {
-  if constexpr (VEC > 1) {
-    if (pieces <= 64) f(Shape<VEC, 64, 1>{});
-    else if (few && pieces <= 256) f(Shape<VEC, 256, 1>{});
-    else if (pieces <= 128) f(Shape<VEC, 64, 2>{});
-    else if (pieces <= 256) f(Shape<VEC, 64, 4>{});
-    else if (pieces <= 512) f(Shape<VEC, 256, 2>{});
-    else if (pieces <= 1024) f(Shape<VEC, 256, 4>{});
-    else if (pieces <= 2048) f(Shape<VEC, 1024, 2>{});
-    else return false;
-  } else {
-    if (pieces <= 256) f(Shape<1, 64, 4>{});
-    else if (pieces <= 1024) f(Shape<1, 256, 4>{});
-    else if (pieces <= 4096) f(Shape<1, 256, 16>{});
-    else if (pieces <= 8192) f(Shape<1, 1024, 8>{});
-    else return false;
-  }
+// The threads of a row and the pieces of a thread (16 bytes: 4 floats or 8 bf16 values), so that a thread holds at most 32 elements: a
+// wave a row while that is enough (no barrier, four rows a workgroup), then 256 or 1024 threads.  `few`: rows that leave most of the chip
+// idle take 256 threads at once.  Rows shorter than a piece go element by element.  False: the row does not fit.
+template <int VEC, typename F> bool with_shape(int dim, bool few, F f) {
+  const int pieces = (dim + VEC - 1) / VEC;
+  if (dim < VEC) f(Shape<1, 64, 1>{});
+  else if (pieces <= 64) f(Shape<VEC, 64, 1>{});
+  else if (few && pieces <= 256) f(Shape<VEC, 256, 1>{});
+  else if (pieces <= 128) f(Shape<VEC, 64, 2>{});
+  else if (pieces <= 256) f(Shape<VEC, 64, 4>{});
+  else if (pieces <= 512) f(Shape<VEC, 256, 2>{});
+  else if (pieces <= 1024) f(Shape<VEC, 256, 4>{});
+  else if (pieces <= 2048) f(Shape<VEC, 1024, 2>{});
+  else return false;
   return true;
 }
-template <typename F> bool with_vec(const RmsNormArgs& a, bool vec, bool few, F f) {
-  // (a piece is 16 bytes: 4 floats or 8 bf16 values; or one element where rows or sizes are not aligned for that)
-  if (a.bf16) return vec ? with_shape<8>(a.dim / 8, few, [&](auto s) { f(uint16_t{}, s); }) : with_shape<1>(a.dim, few, [&](auto s) { f(uint16_t{}, s); });
-  return vec ? with_shape<4>(a.dim / 4, few, [&](auto s) { f(float{}, s); }) : with_shape<1>(a.dim, few, [&](auto s) { f(float{}, s); });
+template <typename F> bool with_type(const RmsNormArgs& a, F f) {
+  const bool few = a.rows <= 1024;
+  if (a.bf16) return with_shape<8>(a.dim, few, [&](auto s) { f(uint16_t{}, s); });
+  return with_shape<4>(a.dim, few, [&](auto s) { f(float{}, s); });
 }
-bool aligned(const RmsNormArgs& a) {
-  const int per = a.bf16 ? 8 : 4;
-  const uintptr_t all = (uintptr_t)a.x | (uintptr_t)a.res | (uintptr_t)a.dy | (uintptr_t)a.dh | (uintptr_t)a.w | (uintptr_t)a.y | (uintptr_t)a.h | (uintptr_t)a.part;
-  return all % 16 == 0 && (a.dim | a.ld_x | (a.res ? a.ld_res : 0) | (a.dy ? a.ld_dy : 0) | (a.dh ? a.ld_dh : 0)) % per == 0;
-}
-bool few_rows(const RmsNormArgs& a) { return a.rows <= 1024; }
 bool bad(const RmsNormArgs* a) {
   return !a || !a->x || !a->w || !a->y || a->rows <= 0 || a->dim <= 0 || a->rows > 0x7fffffffL || a->ld_x < 0 || a->ld_res < 0 || a->ld_dy < 0 || a->ld_dh < 0;
 }
@@ -400,7 +384,7 @@ bool bad(const RmsNormArgs* a) {
 DTF_API int dtf_rms_norm_fwd(const RmsNormArgs* p, hipStream_t st) {
   if (bad(p) || (p->res && !p->h)) return ERR;
   const RmsNormArgs a = *p;
-  const bool done = with_vec(a, aligned(a), few_rows(a), [&](auto type, auto s) {
+  const bool done = with_type(a, [&](auto type, auto s) {
     using T = decltype(type);
     using S = decltype(s);
     constexpr int RPB = S::NT < 256 ? 256 / S::NT : 1, BT = S::NT < 256 ? 256 : S::NT;
@@ -443,7 +427,7 @@ DTF_API int dtf_rms_norm_bwd_blocks(long rows, int dim) {
 DTF_API int dtf_rms_norm_bwd(const RmsNormArgs* p, hipStream_t st) {
   if (bad(p) || !p->dy || !p->rstd || p->blocks != dtf_rms_norm_bwd_blocks(p->rows, p->dim) || (p->dw && p->blocks && !p->part)) return ERR;
   const RmsNormArgs a = *p;
-  const bool done = with_vec(a, aligned(a), few_rows(a), [&](auto type, auto s) {
+  const bool done = with_type(a, [&](auto type, auto s) {
     using T = decltype(type);
     using S = decltype(s);
     const dim3 block(S::NT < 256 ? 256 : S::NT);
