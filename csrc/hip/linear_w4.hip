@@ -86,6 +86,17 @@ __device__ __forceinline__ bf16x8 e2m1_bf16(uint32_t w) {  // eight codes, the l
                                                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 3))));
 }
 
+// v as the lane g of each four lanes holds it (NG: how many of the four hold different values)
+template <int NG> __device__ __forceinline__ uint32_t from_lane_of_four(uint32_t v, int g) {
+  if constexpr (NG == 1) return v;
+  switch (g) {
+    case 0: return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x00, 0xf, 0xf, true);
+    case 1: return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x55, 0xf, 0xf, true);
+    case 2: return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xaa, 0xf, 0xf, true);
+    default: return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xff, 0xf, 0xf, true);
+  }
+}
+
 // GJ: matrix instructions (32 k each) that share a scale; R: tiles of 16 outputs a wave
 template <int XT, int GJ, int R> __global__ __launch_bounds__(512) void linear_w4_kernel(const LinearW4Args a) {
   using T = typename XType<XT>::T;
@@ -101,21 +112,20 @@ template <int XT, int GJ, int R> __global__ __launch_bounds__(512) void linear_w
   for (int r = 0; r < R; ++r) {
     const long nt = min(nt0 + r, nt_all - 1);
     wq[r] = static_cast<const uint4*>(a.wq) + nt * kt_all * 64 + lane;
-    sc[r] = a.scales + nt * kt_all * NG * 16 + 4 * kb;
+    sc[r] = a.scales + (nt * kt_all * NG + col % NG) * 16 + 4 * kb;  // (the tile's groups are shared out over each four lanes)
   }
   f32x4 acc[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
   struct Weights {
     uint4 w[R];
-    uint2 s[R][NG];
+    uint2 s[R];
   };
   auto load = [&](Weights& t, int kt) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       t.w[r] = wq[r][(long)kt * 64];
-#pragma unroll
-      for (int g = 0; g < NG; ++g) t.s[r][g] = *reinterpret_cast<const uint2*>(sc[r] + ((long)kt * NG + g) * 16);
+      t.s[r] = *reinterpret_cast<const uint2*>(sc[r] + (long)kt * NG * 16);
     }
   };
   auto multiply = [&](const Weights& t, const XRaw<XT> (&x)[4]) {
@@ -130,7 +140,7 @@ template <int XT, int GJ, int R> __global__ __launch_bounds__(512) void linear_w
 #pragma unroll
         for (int j = g * GJ; j < (g + 1) * GJ; ++j)
           d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e2m1_bf16(reinterpret_cast<const uint32_t*>(&t.w[r])[j]), b[j], d, 0, 0, 0);
-        const uint2 q = t.s[r][g];
+        const uint2 q = make_uint2(from_lane_of_four<NG>(t.s[r].x, g), from_lane_of_four<NG>(t.s[r].y, g));
         const float s4[4] = {__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u), __uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u)};
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[r][i] = fmaf(d[i], s4[i], acc[r][i]);
