@@ -381,9 +381,7 @@ bool bad(const RmsNormArgs* a) {
 }
 }  // namespace
 
-DTF_API int dtf_rms_norm_fwd(const RmsNormArgs* p, hipStream_t st) {
-  if (bad(p) || (p->res && !p->h)) return ERR;
-  const RmsNormArgs a = *p;
+static void fwd_rows(const RmsNormArgs& a, hipStream_t st) {
   const bool done = with_type(a, [&](auto type, auto s) {
     using T = decltype(type);
     using S = decltype(s);
@@ -411,7 +409,25 @@ DTF_API int dtf_rms_norm_fwd(const RmsNormArgs* p, hipStream_t st) {
     };
     if (a.bf16) go(uint16_t{}); else go(float{});
   }
-  DTF_CHECK_LAUNCH();
+}
+
+DTF_API int dtf_rms_norm_fwd(const RmsNormArgs* p, hipStream_t st) {
+  if (bad(p) || (p->res && !p->h)) return ERR;
+  constexpr long MOST = 1L << 21;  // rows of a launch: its threads have to be fewer than 2^32
+  const long size = p->bf16 ? 2 : 4;
+  const auto skip = [](auto* q, long bytes) { return q ? (decltype(q))((uintptr_t)q + bytes) : q; };
+  for (long r = 0; r < p->rows; r += MOST) {
+    RmsNormArgs a = *p;
+    a.rows = p->rows - r < MOST ? p->rows - r : MOST;
+    a.x = skip(a.x, r * a.ld_x * size);
+    a.res = skip(a.res, r * a.ld_res * size);
+    a.h = skip(a.h, r * a.dim * size);
+    a.y = skip(a.y, r * a.dim * (a.q_scale ? 1 : size));
+    a.rstd = skip(a.rstd, r * 4);
+    a.q_scale = skip(a.q_scale, r * 4);
+    fwd_rows(a, st);
+    DTF_CHECK_LAUNCH();
+  }
   return 0;
 }
 

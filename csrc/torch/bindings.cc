@@ -22,8 +22,11 @@ using OptTensor = std::optional<Tensor>;
 namespace {
 
 hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+struct NativeError : std::runtime_error {  // native.NativeError on the Python side
+  using std::runtime_error::runtime_error;
+};
 void check(int rc, const char* what) {
-  TORCH_CHECK(rc == 0, what, " failed with code ", rc, rc == -22 ? " (shape/alignment precondition violated)" : "");
+  if (rc != 0) throw NativeError(c10::str(what, " failed with code ", rc, rc == -22 ? " (shape/alignment precondition violated)" : ""));
 }
 bool is_rows(const Tensor& t) {
   return t.is_cuda() && t.layout() == at::kStrided && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) && t.dim() >= 1;
@@ -323,7 +326,7 @@ struct AdamWGroup {
     const c10::DeviceGuard guard(params[0].device());
     const int rc = dtf_adamw(&a, pp.data(), gg.data(), kind.data(), stream_of(params[0]));
     for (size_t i = 0; i < grads.size(); ++i)
-      if (grads[i].defined()) params[i].unsafeGetTensorImpl()->bump_version();  // (a backward pass that saved the old values is refused)
+      if (grads[i].defined() && !params[i].is_inference()) params[i].unsafeGetTensorImpl()->bump_version();  // (a backward pass that saved the old values is refused)
     grads.clear();
     check(rc, "adamw");
   }
@@ -332,7 +335,14 @@ struct AdamWGroup {
 }  // namespace
 
 PYBIND11_MODULE(libdtf_torch, m) {
-  m.attr("W4_MAX_ROWS") = W4_MAX_ROWS;
+  static const py::object error = py::module_::import("distributed_tensorflow_amd.native").attr("NativeError");
+  py::register_exception_translator([](std::exception_ptr p) {
+    try {
+      if (p) std::rethrow_exception(p);
+    } catch (const NativeError& e) {
+      PyErr_SetString(error.ptr(), e.what());
+    }
+  });
   m.def("rms_norm_forward", &rms_norm_forward);
   m.def("rms_norm_e4m3", &rms_norm_e4m3);
   m.def("rms_norm_backward", &rms_norm_backward);

@@ -126,7 +126,8 @@ def _recipe(which: str):
         import torch
         d, home = os.path.join(CSRC, "torch"), os.path.dirname(torch.__file__)
         rocm = os.path.dirname(os.path.dirname(HIPCC))
-        cc = [CXX, "-O2", "-fPIC", "-std=c++17", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"]
+        cc = [CXX, "-O2", "-fPIC", "-std=c++17", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+              "-DDTF_TORCH=" + torch.__version__]  # (part of the digest: another torch needs another build)
         for i in (home + "/include", home + "/include/torch/csrc/api/include", rocm + "/include", sysconfig.get_paths()["include"]):
             cc += ["-isystem", i]
         cc += ["-I", os.path.join(CSRC, "hip")]

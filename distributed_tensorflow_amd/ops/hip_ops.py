@@ -352,6 +352,7 @@ def rms_norm_backward(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, wei
 _E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
+@torch.no_grad()
 def quantize_w4(w: torch.Tensor, group: int = 64) -> Tuple[torch.Tensor, torch.Tensor]:
     """fp32 or bf16 weights ``w[K,N]`` -> ``(wq, scales)`` for ``linear_w4``, on any device; ``group``: 32, 64 or 128 successive k share a scale.
 
@@ -394,6 +395,7 @@ def _w4_group(wq: torch.Tensor, scales: torch.Tensor) -> int:
     return wq.shape[1] * 128 // scales.shape[1]
 
 
+@torch.no_grad()
 def dequantize_w4(wq: torch.Tensor, scales: torch.Tensor, in_features: int, out_features: int) -> torch.Tensor:
     """The fp32 weights ``[in_features, out_features]`` that ``quantize_w4``'s result stands for."""
     group = _w4_group(wq, scales)

@@ -203,7 +203,7 @@ class AdamW(torch.optim.Optimizer):
         """The group's live moments: ``m`` and ``v`` (fp32), or ``m`` and ``r`` = sqrt(v) (e4m3) with ``m_scale`` and ``r_scale``, one
         for 256 elements; and the step counters, one a tensor.  Tensor i starts at a multiple of 256 elements."""
         st = self._groups[group]
-        return {**st.arenas, "step": st.step}
+        return {} if st is None else {**st.arenas, "step": st.step}
 
     @torch.no_grad()
     def step(self, closure=None, *, grads: Optional[Sequence[Optional[torch.Tensor]]] = None, grad_scale: float = 1.0):

@@ -154,6 +154,9 @@ def test_groups_added_later_and_empty_tensors():
     assert int(opt.state[a]["step"]) == 1 and opt.state[b]["m"].numel() == 0
     loss = opt.step(lambda: torch.tensor(2.0))
     assert float(loss) == 2.0
+    opt.add_param_group({"params": []})
+    opt.step()
+    assert opt.arenas(2) == {} and int(opt.state[a]["step"]) == 3
 
 
 def test_refusals_change_nothing():

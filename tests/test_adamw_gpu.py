@@ -171,6 +171,24 @@ def test_places_behind_two_to_the_31():
     assert not p.detach()[5000:lo].any() and not opt.arenas()["m"].view(torch.uint8)[5120:lo].any()
 
 
+def test_schedulers_and_a_tensor_changed_behind_the_optimizers_back():
+    p = torch.ones(100, device="cuda", requires_grad=True)
+    opt = AdamW([p], lr=1.0, weight_decay=0.0, eps=0.0)
+    sched = torch.optim.lr_scheduler.StepLR(opt, 1, gamma=0.5)
+    for want in (0.0, -0.5):  # the first steps of a constant gradient are lr long
+        p.grad = torch.ones(100, device="cuda")
+        opt.step()
+        sched.step()
+        assert bool(((p.detach() - want).abs() <= 16 * 2.0 ** -24).all())
+    loss = (p * p).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    p.data = p.data.to(B)
+    with pytest.raises(ValueError, match="has changed"):
+        opt.step(grads=[torch.ones(100, device="cuda")])
+
+
 def test_refusals_on_the_gpu():
     p = torch.zeros(8, device="cuda", requires_grad=True)
     with pytest.raises(ValueError, match="one device"):

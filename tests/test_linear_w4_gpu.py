@@ -142,6 +142,34 @@ def test_layers_capture_and_another_stream():
     assert torch.equal(y, z)
 
 
+def test_weights_behind_two_to_the_32_bytes():
+    from distributed_tensorflow_amd.ops import hip_ops
+    K, N = 65600, 140001
+    kt, nt = -(-K // 128), -(-N // 16)
+    gen = torch.Generator("cuda").manual_seed(0)
+    wq = torch.randint(0, 256, (nt, kt, 64, 16), generator=gen, device="cuda", dtype=torch.uint8)
+    scales = torch.rand(nt, kt * 4, 16, generator=gen, device="cuda").to(B)
+    assert wq.numel() > 1 << 32
+    x, _ = _rows(2, K, B)
+    y = hip_ops.linear_w4(x, wq, scales, N)
+    for lo, hi in ((0, 2), (nt - 2, nt)):  # the first and the last outputs
+        w = hip_ops.dequantize_w4(wq[lo:hi], scales[lo:hi], K, 32).double()[:, :min(N, hi * 16) - lo * 16]
+        check(y[:, lo * 16:hi * 16], x, None, w, None, False)
+
+
+def test_e4m3_nan_and_gradients_that_are_not_taken():
+    from distributed_tensorflow_amd.ops import hip_ops
+    w = torch.randn(64, 32, device="cuda", requires_grad=True)
+    wq, scales = hip_ops.quantize_w4(w)
+    assert not scales.requires_grad and not hip_ops.dequantize_w4(wq, scales, 64, 32).requires_grad
+    x = torch.ones(2, 64, device="cuda")
+    x[1, 3] = float("nan")
+    y = hip_ops.linear_w4(x.to(E), wq, scales, 32, x_scale=torch.ones(2, device="cuda"))
+    assert bool(torch.isfinite(y[0]).all()) and bool(torch.isnan(y[1]).all())
+    y = hip_ops.linear_w4(x[:1].to(E), wq, scales, 32, x_scale=torch.zeros(1, device="cuda"), bias=torch.ones(32, device="cuda"))
+    assert bool((y == 1).all())
+
+
 def test_empty_batches_and_refusals():
     from distributed_tensorflow_amd.ops import hip_ops
     wq, scales, _ = _weights(64, 32, 64)

@@ -212,6 +212,35 @@ def test_rows_behind_two_to_the_31_elements():
     check_e4m3(q[-5:], scale[-5:], x[-5:], w, None, 1e-6)
 
 
+def test_more_rows_than_a_launch_takes():
+    from distributed_tensorflow_amd.ops import hip_ops
+    rows = (1 << 21) + 1000
+    x = torch.randn(rows, 24, generator=torch.Generator("cuda").manual_seed(0), device="cuda")
+    w = torch.ones(24, device="cuda")
+    y, h, rstd = hip_ops.rms_norm_forward(x, w, x)
+    check_forward(y, h, rstd, x, w, x, 1e-6)
+    q, scale, h2 = hip_ops.rms_norm_e4m3(x.to(B), w, x.to(B))
+    check_e4m3(q, scale, x.to(B), w, x.to(B), 1e-6)
+    dx, dw = hip_ops.rms_norm_backward(x, x, rstd, w, x)
+    check_backward(dx, dw, x, x, rstd, w, x, None)
+
+
+def test_a_single_row_without_a_batch_and_inference_mode():
+    from distributed_tensorflow_amd.ops import autograd, hip_ops
+    x = torch.randn(300, device="cuda")
+    w = torch.rand(300, device="cuda", requires_grad=True)
+    y, h, rstd = hip_ops.rms_norm_forward(x, w)
+    assert y.shape == (300,) and rstd.shape == () and not y.requires_grad
+    check_forward(y, h, rstd, x, w.detach(), None, 1e-6)
+    dx, dw = hip_ops.rms_norm_backward(y, x, rstd, w)
+    check_backward(dx, dw, y, x, rstd, w.detach(), None, None)
+    q, scale, _ = hip_ops.rms_norm_e4m3(x, w)
+    assert q.shape == (300,) and scale.shape == ()
+    with torch.inference_mode():
+        a, b = autograd.rms_norm(x, w, x)
+        assert torch.equal(b, x + x) and not a.requires_grad
+
+
 def test_refusals():
     from distributed_tensorflow_amd.ops import hip_ops
     x, w = torch.zeros(4, 8, device="cuda"), torch.ones(8, device="cuda")
