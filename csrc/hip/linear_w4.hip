@@ -5,7 +5,8 @@
 // v_mfma_f32_16x16x32_bf16 take it: A = the weights, turned into bf16 two at a time by v_cvt_scalef32_pk_bf16_fp4 (0, 0.5 .. 6 are exact),
 // B = up to 16 rows of x.  With a single row 15 columns of B are idle, which costs nothing: the instruction is not what bounds the kernel,
 // and unpacking to fp32 for vector FMAs would need three times the VALU work.  The group's scales are applied in fp32 to the
-// accumulator of the group (G = 32, 64, 128: 1, 2, 4 instructions).
+// accumulator of the group (G = 32, 64, 128: 1, 2, 4 instructions).  16384 x 16384 take 28-29 us for 1 row (bf16, G = 64) and 16 (e4m3,
+// G = 128): 4.9 TB/s of weights, where a large copy reaches 5.1.
 //
 // x: bf16; e4m3 (exact in bf16) with a scale a row; or fp32, each row as three columns of B, x = hi + mid + lo in bf16 by cutting the
 // mantissa (8 + 8 + 8 bits: the sum is exact), added up at the end: fp32 rows lose nothing to the matrix instruction's type.
@@ -26,58 +27,47 @@ template <> struct XType<X_E4M3> { using T = uint8_t; static constexpr int P = 1
 __device__ __forceinline__ uint32_t word_of(float e) { return __float_as_uint(e); }
 __device__ __forceinline__ uint32_t word_of(uint16_t e) { return e; }
 __device__ __forceinline__ uint32_t word_of(uint8_t e) { return e; }
-// eight consecutive k of a row as loaded
-template <int XT> struct XRaw { uint32_t w[2 * sizeof(typename XType<XT>::T)]; };
-template <int XT> __device__ __forceinline__ XRaw<XT> x_load(const typename XType<XT>::T* p) {
-  XRaw<XT> r;
-  __builtin_memcpy(&r, p, sizeof(r));  // (wide loads also where a row starts at an odd element)
-  return r;
-}
-// the same where the row ends among or before them: zeros from there on, nothing behind the row is read
-template <int XT> __device__ __forceinline__ XRaw<XT> x_load_end(const typename XType<XT>::T* row, int k, int K) {
-  using T = typename XType<XT>::T;
-  constexpr int PER = 4 / sizeof(T);  // elements a word
-  XRaw<XT> r;
-#pragma unroll
-  for (int i = 0; i < (int)(2 * sizeof(T)); ++i) {
-    r.w[i] = 0;
-#pragma unroll
-    for (int h = 0; h < PER; ++h) {
-      const int at = k + i * PER + h;
-      const T e = row[min(at, K - 1)];
-      r.w[i] |= at < K ? word_of(e) << (8 * (int)sizeof(T) * h) : 0u;
-    }
-  }
-  return r;
-}
-// as bf16; fp32: the part of x that column `plane` of the three takes
-template <int XT> __device__ __forceinline__ bf16x8 x_bf16(const XRaw<XT>& r, int plane) {
-  uint32_t u[4];
+// 16 bytes of a row: 4, 8 or 16 elements
+struct XPiece {
+  uint32_t w[4];
+};
+// A tile of x (the rows of this pass x 128 k) goes through LDS: the wave loads it in one piece, 16 bytes a lane, turns it into bf16 and
+// writes it as the columns of B; then every lane reads its parts of its column.  Loaded from memory in B's order, a lane's column at a time,
+// few rows are read by up to 16 lanes each (and converted as often), and the load unit, not memory, is what bounds the kernel.
+// PITCH: 16 columns' parts of 16 bytes fall into all 64 banks.
+constexpr int PITCH = 128 + 8;
+template <int XT> __device__ __forceinline__ void store_columns(uint16_t* tile, int row, int k, const XPiece& x) {
   if constexpr (XT == X_BF16) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = r.w[i];
+    *reinterpret_cast<uint4*>(tile + row * PITCH + k) = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
   } else if constexpr (XT == X_E4M3) {
+    uint32_t u[8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      u[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.w[i], 1.f, false));
-      u[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(r.w[i], 1.f, true));
+    for (int i = 0; i < 4; ++i) {
+      u[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.w[i], 1.f, false));
+      u[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x.w[i], 1.f, true));
     }
+    uint4* to = reinterpret_cast<uint4*>(tile + row * PITCH + k);
+    to[0] = make_uint4(u[0], u[1], u[2], u[3]);
+    to[1] = make_uint4(u[4], u[5], u[6], u[7]);
   } else {
-    // the upper 16 bits are taken off as often as the plane's number says (masks instead of branches: the planes are a wave's lanes).
-    // Both differences are exact.  Column 0 takes a NaN or an infinity as it is (the difference with 0 makes a NaN quiet, so that one
-    // whose bits all lie in the lower half survives); infinity less itself, a NaN, is none of the others' business.
-    const uint32_t once = plane >= 1 ? 0xffff0000u : 0u, twice = plane >= 2 ? 0xffff0000u : 0u;
-    float part[8];
+    // the upper 16 bits, those of the rest, and what is left: both differences are exact.  The first column takes a NaN or an infinity (a
+    // NaN made quiet, so that one whose bits all lie in the lower half survives); infinity less itself, a NaN, is none of the others' business.
+    uint32_t part[3][4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = __uint_as_float(r.w[i]), y = x - __uint_as_float(r.w[i] & once);
-      part[i] = y - __uint_as_float(__float_as_uint(y) & twice);
-      part[i] = plane >= 1 && part[i] != part[i] ? 0.f : part[i];
+    for (int i = 0; i < 4; ++i) {
+      const float v = __uint_as_float(x.w[i]);
+      const uint32_t bits = x.w[i], nan = v != v ? 0x00400000u : 0u;
+      float rest = v - __uint_as_float(bits & 0xffff0000u);
+      rest = rest == rest ? rest : 0.f;
+      part[0][i] = bits | nan;
+      part[1][i] = __float_as_uint(rest);
+      part[2][i] = __float_as_uint(rest - __uint_as_float(part[1][i] & 0xffff0000u));
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = (__float_as_uint(part[2 * i]) >> 16) | (__float_as_uint(part[2 * i + 1]) & 0xffff0000u);
+    for (int p = 0; p < 3; ++p)
+      *reinterpret_cast<uint2*>(tile + (3 * row + p) * PITCH + k) =
+          make_uint2((part[p][0] >> 16) | (part[p][1] & 0xffff0000u), (part[p][2] >> 16) | (part[p][3] & 0xffff0000u));
   }
-  return __builtin_bit_cast(bf16x8, make_uint4(u[0], u[1], u[2], u[3]));
 }
 __device__ __forceinline__ bf16x8 e2m1_bf16(uint32_t w) {  // eight codes, the low nibble of the low byte first
   return __builtin_bit_cast(bf16x8, make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.f, 0)),
@@ -97,15 +87,19 @@ template <int NG> __device__ __forceinline__ uint32_t from_lane_of_four(uint32_t
   }
 }
 
-// GJ: matrix instructions (32 k each) that share a scale; R: tiles of 16 outputs a wave
-template <int XT, int GJ, int R> __global__ __launch_bounds__(512) void linear_w4_kernel(const LinearW4Args a) {
+// GJ: matrix instructions (32 k each) that share a scale; R: tiles of 16 outputs a wave; PIECES: of x a lane, one for few rows
+template <int XT, int GJ, int R, int PIECES> __global__ __launch_bounds__(512) void linear_w4_kernel(const LinearW4Args a) {
   using T = typename XType<XT>::T;
   constexpr int P = XType<XT>::P, MC = 16 / P, NG = 4 / GJ;
-  extern __shared__ __attribute__((aligned(16))) float part[];  // [waves][R][16 n][16 columns]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, kb = lane >> 4, col = lane & 15;
-  const int nt_all = (a.N + 15) / 16, kt_all = (a.K + 127) / 128, nt0 = blockIdx.x * R, plane = col % P;
-  const long m0 = (long)blockIdx.y * MC, mine = min(m0 + col / P, a.M - 1);  // (columns behind the last row repeat it: not stored)
-  const T* row = static_cast<const T*>(a.x) + mine * a.ldx;
+  constexpr int E = 16 / sizeof(T), PER_ROW = 128 / E;  // elements of a piece, pieces of a row
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // a tile of x for each wave; at the end [waves][R][16 n][16 columns] sums
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, kb = lane >> 4, col = lane & 15;
+  const int nt_all = (a.N + 15) / 16, kt_all = (a.K + 127) / 128, nt0 = blockIdx.x * R;
+  const long m0 = (long)blockIdx.y * MC;
+  const int rows = (int)min((long)MC, a.M - m0);  // of this pass
+  const T* const x0 = static_cast<const T*>(a.x) + m0 * a.ldx;
+  uint16_t* const tile = reinterpret_cast<uint16_t*>(lds) + wave * 16 * PITCH;
+  const uint16_t* const column = tile + min(col, rows * P - 1) * PITCH + 8 * kb;  // (columns behind the last repeat it: not stored)
   const uint4* wq[R];
   const uint16_t* sc[R];
 #pragma unroll
@@ -128,10 +122,18 @@ template <int XT, int GJ, int R> __global__ __launch_bounds__(512) void linear_w
       t.s[r] = *reinterpret_cast<const uint2*>(sc[r] + (long)kt * NG * 16);
     }
   };
-  auto multiply = [&](const Weights& t, const XRaw<XT> (&x)[4]) {
+  auto multiply = [&](const Weights& t, const XPiece (&x)[PIECES]) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int c = i * 64 + lane;
+      store_columns<XT>(tile, min(c / PER_ROW, MC - 1), c % PER_ROW * E, x[i]);  // (rows behind the last hold it again)
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (a wave's own tile: its LDS accesses are done in order)
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     bf16x8 b[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) b[j] = x_bf16<XT>(x[j], plane);
+    for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const bf16x8*>(column + 32 * j);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -146,27 +148,52 @@ template <int XT, int GJ, int R> __global__ __launch_bounds__(512) void linear_w
         for (int i = 0; i < 4; ++i) acc[r][i] = fmaf(d[i], s4[i], acc[r][i]);
       }
   };
-  // Whole tiles of k.  All loads of a tile are on their way before the first is waited for (left to itself the compiler puts each load of x
-  // next to its use, a round trip to the caches each: 17 us instead of 9.5 for one row of 16384 by 2048 outputs).  Two tiles at a time
-  // gained nothing further: eight to sixteen waves a CU hide the rest.
+  // Whole tiles of k; the next tile's loads are on their way while one is multiplied.
   const int whole = a.K / 128;
-  for (int kt = wave; kt < whole; kt += waves) {
-    Weights t;
-    XRaw<XT> x[4];
+  auto fetch = [&](Weights& t, XPiece (&x)[PIECES], int kt) {
     load(t, kt);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = x_load<XT>(row + kt * 128 + 32 * j + 8 * kb);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(t, x);
+    for (int i = 0; i < PIECES; ++i) {
+      const int c = i * 64 + lane;
+      __builtin_memcpy(&x[i], x0 + min(c / PER_ROW, rows - 1) * a.ldx + kt * 128 + c % PER_ROW * E, 16);
+    }
+  };
+  if (wave < whole) {
+    Weights t, t2;
+    XPiece x[PIECES], x2[PIECES];
+    fetch(t, x, wave);
+    for (int kt = wave; kt < whole; kt += 2 * waves) {
+      // (behind the end: this one again, not multiplied.  Without a branch, so that the compiler counts the loads that are still out and
+      // waits for the older half alone: behind a branch it waits for all, 8.9 instead of 7.6 us for one row of 16384 by 2048 outputs)
+      fetch(t2, x2, kt + waves < whole ? kt + waves : kt);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(t, x);
+      __builtin_amdgcn_wave_barrier();
+      fetch(t, x, kt + 2 * waves < whole ? kt + 2 * waves : kt);
+      __builtin_amdgcn_sched_barrier(0);
+      if (kt + waves < whole) multiply(t2, x2);
+      __builtin_amdgcn_wave_barrier();
+    }
   }
-  if (whole < kt_all && wave == whole % waves) {  // the rest of k
+  if (whole < kt_all && wave == whole % waves) {  // the rest of k: zeros behind it, nothing behind a row's end is read
     Weights t;
-    XRaw<XT> x[4];
+    XPiece x[PIECES];
     load(t, whole);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = x_load_end<XT>(row, whole * 128 + 32 * j + 8 * kb, a.K);
+    for (int i = 0; i < PIECES; ++i) {
+      const int c = i * 64 + lane, k = whole * 128 + c % PER_ROW * E;
+      const T* row = x0 + min(c / PER_ROW, rows - 1) * a.ldx;
+#pragma unroll
+      for (int h = 0; h < E; ++h) {
+        const uint32_t e = word_of(row[min(k + h, a.K - 1)]) << (8 * (int)sizeof(T) * (h % (4 / (int)sizeof(T))));
+        uint32_t& to = x[i].w[h / (4 / (int)sizeof(T))];
+        to = (h % (4 / (int)sizeof(T)) ? to : 0u) | (k + h < a.K ? e : 0u);
+      }
+    }
     multiply(t, x);
   }
+  __syncthreads();
+  float* const part = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -191,15 +218,20 @@ template <int XT, int GJ, int R> __global__ __launch_bounds__(512) void linear_w
 
 namespace {
 template <int XT, int GJ, int R> void go(const LinearW4Args& a, int passes, hipStream_t st) {
-  // eight waves split k (16 were as fast at best; 4 took 9 instead of 7 us where 65 workgroups share 25 tiles of k, and are even elsewhere)
+  constexpr int ROW = 128 * sizeof(typename XType<XT>::T), MC = 16 / XType<XT>::P, MOST = (MC * ROW + 1023) / 1024;  // bytes of a tile's row; KB of a tile
+  // eight waves split k (4: 15.2 instead of 9.1 us for one row of 16384 by 2048 outputs; 16: 10.3, and even elsewhere)
   const int nt = (a.N + 15) / 16, kt = (a.K + 127) / 128, waves = kt < 8 ? kt : 8;
-  hipLaunchKernelGGL((linear_w4_kernel<XT, GJ, R>), dim3((nt + R - 1) / R, passes), dim3(64 * waves), sizeof(float) * waves * R * 256, st, a);
+  const dim3 grid((nt + R - 1) / R, passes);
+  static_assert(32 * PITCH >= R * 1024, "a wave's sums take the place of its tile of x");
+  const int lds = 32 * PITCH * waves;
+  if (a.M * ROW <= 1024) hipLaunchKernelGGL((linear_w4_kernel<XT, GJ, R, 1>), grid, dim3(64 * waves), lds, st, a);
+  else hipLaunchKernelGGL((linear_w4_kernel<XT, GJ, R, MOST>), grid, dim3(64 * waves), lds, st, a);
 }
-// More rows than the columns of B hold (16; fp32 5) take a pass over the weights for each such set, side by side in one launch: several
-// column tiles a wave were slower, because x is what a wave reads most (16 rows of bf16 are four times a tile's weights): 64 rows of bf16,
-// 4096 x 16384: 30.6 us, with four column tiles a wave 35.5.  For the same reason the tiles of outputs a wave takes are as many as leave
-// the chip filled.  Measured, us with 1 / 2 / 4 tiles, by tiles of outputs x passes (k 4096): 256 (2048 outputs, 32 rows bf16) 6.8 / 8.2 / 10.5;
-// 512 (8192, 16 rows bf16) 11.2 / 8.6 / 10.7; 1024 (16384, 16 rows bf16) 19.5 / 13.4 / 11.3, (16384, 5 rows fp32) 20.2 / 14.1 / 13.0.
+// More rows than the columns of B hold (16; fp32 5) take a pass over the weights for each such set, side by side in one launch (several
+// column tiles a wave were slower: 64 rows bf16, 4096 x 16384, 35.5 instead of 30.6 us).  A wave takes as many tiles of outputs as leave the
+// chip filled, because each tile of x is then loaded and turned less often.  Measured, us with 1 / 2 / 4 tiles, by tiles of outputs x passes:
+// 256 (16 rows bf16, 4096 x 4096) 4.8 / 6.0 / 8.7; 512 (1 row bf16, 8192 x 8192) 8.1 / 8.0 / 9.9, (5 rows fp32) 14.0 / 11.1 / 15.1; 750 (16 rows
+// bf16, 4096 x 12000) 9.8 / 10.5 / 9.9; 1024 (16 rows e4m3, 16384 x 16384) 39.1 / 31.6 / 28.9, (1 row bf16) 28.6 / 27.3 / 28.2.
 template <int XT, int GJ> void with_tiles(const LinearW4Args& a, hipStream_t st) {
   constexpr int MC = 16 / XType<XT>::P;
   const int passes = (int)((a.M + MC - 1) / MC);
