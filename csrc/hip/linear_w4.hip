@@ -31,6 +31,35 @@ __device__ __forceinline__ uint32_t word_of(uint8_t e) { return e; }
 struct XPiece {
   uint32_t w[4];
 };
+// The piece at k of a row of K elements, zeros behind its end.  One that reaches over the end is loaded as the row's last 16 bytes and
+// shifted into place; a row shorter than that goes element by element.
+template <typename T> __device__ __forceinline__ XPiece last_piece(const T* row, int k, int K) {
+  constexpr int E = 16 / sizeof(T), PER = 4 / sizeof(T);
+  XPiece x;
+  if (K >= E) {
+    uint64_t h[2];
+    __builtin_memcpy(h, row + min(k, K - E), 16);
+    const int over = max(k - (K - E), 0) * 8 * (int)sizeof(T);  // bits to drop at the low end
+    const uint64_t lo = over >= 64 ? h[1] >> (over & 63) : over ? h[0] >> over | h[1] << (64 - over) : h[0];
+    const uint64_t hi = over >= 64 ? 0 : h[1] >> over;
+    const bool in = k < K;
+    x.w[0] = in ? (uint32_t)lo : 0u;
+    x.w[1] = in ? (uint32_t)(lo >> 32) : 0u;
+    x.w[2] = in ? (uint32_t)hi : 0u;
+    x.w[3] = in ? (uint32_t)(hi >> 32) : 0u;
+  } else {
+    T e[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) e[i] = row[min(k + i, K - 1)];
+    __builtin_amdgcn_sched_barrier(0);  // (all loads first)
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const uint32_t v = k + i < K ? word_of(e[i]) << (8 * (int)sizeof(T) * (i % PER)) : 0u;
+      x.w[i / PER] = i % PER ? x.w[i / PER] | v : v;
+    }
+  }
+  return x;
+}
 // A tile of x (the rows of this pass x 128 k) goes through LDS: the wave loads it in one piece, 16 bytes a lane, turns it into bf16 and
 // writes it as the columns of B; then every lane reads its parts of its column.  Loaded from memory in B's order, a lane's column at a time,
 // few rows are read by up to 16 lanes each (and converted as often), and the load unit, not memory, is what bounds the kernel.
@@ -181,14 +210,8 @@ template <int XT, int GJ, int R, int PIECES> __global__ __launch_bounds__(512) v
     load(t, whole);
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int c = i * 64 + lane, k = whole * 128 + c % PER_ROW * E;
-      const T* row = x0 + min(c / PER_ROW, rows - 1) * a.ldx;
-#pragma unroll
-      for (int h = 0; h < E; ++h) {
-        const uint32_t e = word_of(row[min(k + h, a.K - 1)]) << (8 * (int)sizeof(T) * (h % (4 / (int)sizeof(T))));
-        uint32_t& to = x[i].w[h / (4 / (int)sizeof(T))];
-        to = (h % (4 / (int)sizeof(T)) ? to : 0u) | (k + h < a.K ? e : 0u);
-      }
+      const int c = i * 64 + lane;
+      x[i] = last_piece(x0 + min(c / PER_ROW, rows - 1) * a.ldx, whole * 128 + c % PER_ROW * E, a.K);
     }
     multiply(t, x);
   }

@@ -42,7 +42,7 @@ def check(y, x, scale, w, bias, relu):
 
 # (rows, K, N): one element; tails of k and of outputs; one k tile and many; one, two and four tiles of columns; rows behind the last chunk
 SHAPES = [(1, 1, 1), (1, 128, 16), (1, 2048, 1008), (2, 130, 33), (3, 127, 5), (5, 3136, 1025), (6, 96, 40), (10, 256, 48), (11, 264, 16), (16, 512, 64),
-          (17, 1000, 31), (32, 1024, 16), (33, 72, 100), (64, 640, 200), (65, 256, 17), (150, 136, 20), (1, 16384, 8200), (16, 4096, 8208)]
+          (17, 1000, 31), (32, 1024, 16), (33, 72, 100), (64, 640, 200), (65, 256, 17), (150, 136, 20), (3, 2, 20), (4, 9, 17), (2, 15, 3), (16, 141, 16), (5, 2047, 40), (1, 16384, 8200), (16, 4096, 8208)]
 
 
 @pytest.mark.parametrize("dtype", [F, B, E])
