@@ -9,6 +9,10 @@
 // address from one call to the next), advances every tensor's step counter and works out its bias corrections; `apply` runs over a
 // fixed list of 2048-element chunks of all tensors.
 //
+// Measured: 190 tensors of 24 M fp32 elements, 8-bit moments, 72 us (5.3 TB/s); 64 of 268 M bf16 elements 494-545 us (5.0-5.5 TB/s), where about
+// 65 issue slots an element keep the vector units two thirds busy (at 105, before the conversion and the root were shortened, they were
+// the bound: 678 us); MNIST's eight tensors with 32-bit moments 18.5 us (5.0 TB/s).
+//
 // 8-bit moments: 256 elements share a scale.  m and r = sqrt(v) (the root halves the range that the code has to span) are e4m3 times
 // a power of two that brings the block's largest magnitude into [128, 256).  They are rounded stochastically, with 16 bits of a hash
 // of seed, step, block and element: with b2 = 0.999 one step moves r by 0.05 % of itself and e4m3's grid is 6-12 %, so rounding to
