@@ -273,7 +273,8 @@ template <int XT> void with_group(const LinearW4Args& a, hipStream_t st) {
 DTF_API int dtf_linear_w4(const LinearW4Args* p, hipStream_t st) {
   if (!p || !p->x || !p->wq || !p->scales || !p->y || p->M <= 0 || p->N <= 0 || p->K <= 0 || p->ldx < 0) return ERR;
   if ((p->group != 32 && p->group != 64 && p->group != 128) || p->xtype < 0 || p->xtype > 2) return ERR;
-  if ((uintptr_t)p->wq % 16 || (uintptr_t)p->scales % 8 || p->M > 65535L * 5) return ERR;  // (grid.y: five rows and more each)
+  if ((uintptr_t)p->wq % 16 || (uintptr_t)p->scales % 8 || p->M > 65535L * 5 || p->K > 0x7fffff00 || p->N > 0x7fffff00)
+    return ERR;  // (grid.y: five rows and more each; sums with a tile stay inside an int)
   if (p->xtype == X_F32) with_group<X_F32>(*p, st);
   else if (p->xtype == X_BF16) with_group<X_BF16>(*p, st);
   else with_group<X_E4M3>(*p, st);

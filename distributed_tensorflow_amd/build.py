@@ -73,7 +73,10 @@ def _sources(srcdir: str, exts) -> List[str]:
 def source_digest(which: str) -> str:
     """Digest of the sources + build line that ``libdtf_<which>.so`` must have been built from."""
     srcdir, exts, cc, ld, _ = _recipe(which)
-    return _digest(_sources(srcdir, exts) + _all_headers(which), " ".join(cc + ld))
+    words = cc + ld
+    if which == "torch":  # (where torch and ROCm are installed does not count, which torch it is does: -DDTF_TORCH)
+        words = [w for w in words if not w.startswith("/") or w.startswith(ROOT) or w == CXX]
+    return _digest(_sources(srcdir, exts) + _all_headers(which), " ".join(words))
 
 
 def _all_headers(which: str) -> List[str]:

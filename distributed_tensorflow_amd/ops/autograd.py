@@ -276,9 +276,11 @@ class LinearW4(nn.Module):
 
     def __init__(self, in_features: int, out_features: int, relu: bool = False, group: int = 64):
         super().__init__()
-        wq, scales = hip_ops.quantize_w4(torch.zeros(in_features, out_features), group)
-        self.register_buffer("wq", wq)
-        self.register_buffer("scales", scales)
+        if group not in (32, 64, 128):
+            raise ValueError("group is 32, 64 or 128 (got %r)" % (group,))
+        nt, kt = -(-out_features // 16), -(-in_features // 128)
+        self.register_buffer("wq", torch.zeros(nt, kt, 64, 16, dtype=torch.uint8))
+        self.register_buffer("scales", torch.zeros(nt, kt * 128 // group, 16, dtype=torch.bfloat16))
         self.register_buffer("bias", torch.zeros(out_features))
         self.in_features, self.out_features, self.relu = in_features, out_features, relu
 

@@ -329,7 +329,8 @@ def rms_norm_forward(x: torch.Tensor, weight: torch.Tensor, residual: Optional[t
     """``h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension -> ``(y, h, rstd)``.
 
     ``x``, ``residual``: fp32 or bf16 rows of one type, any stride between rows; ``weight`` fp32.  ``h`` (``x`` itself without a
-    residual) is rounded to that type, ``y`` comes from the unrounded sum; ``rstd`` (fp32, one a row) is for ``rms_norm_backward``."""
+    residual) is rounded to that type, ``y`` comes from the unrounded sum; ``rstd`` (fp32, one a row) is for ``rms_norm_backward``.
+    Squares are summed in fp32: a row with magnitudes above 1e19 gives zeros."""
     return native.ext().rms_norm_forward(x, weight, residual, eps)
 
 

@@ -60,6 +60,8 @@ def test_refusals():
     layer = autograd.LinearW4.from_linear(autograd.Linear(64, 32))
     with pytest.raises(ValueError, match="CUDA"):
         layer(torch.zeros(1, 64))
+    with pytest.raises(ValueError, match="group"):
+        autograd.LinearW4(64, 32, group=48)
     again = autograd.LinearW4(64, 32)
     again.load_state_dict(layer.state_dict())
     assert torch.equal(again.wq, layer.wq) and torch.equal(again.scales.view(torch.int16), layer.scales.view(torch.int16))
