@@ -309,9 +309,10 @@ class StartupMixin:
                 raise RuntimeError("%s; rank %d: first-step gradients %s; [epoch, errors, ticket, seen, tag, ..] of the "
                                    "exchanges %s; start-up log: %s" % (err, self.rank, ", ".join(seen), words,
                                                                        " | ".join(self.startup_log))) from None
-            # the dropped candidates' expired waits are in the log and the state is the snapshot again: the chosen schedule
-            # starts with a clean count (ensure_healthy() / check_transport() act on ANY expiry since then)
-            if broken:
+            # the trials' expired waits (of dropped candidates, or of a first try that was repeated) are in the log and the state is
+            # the snapshot again: the chosen schedule starts with a clean count (ensure_healthy() / check_transport() act on ANY
+            # expiry since then)
+            if broken or ops.expired_seen:
                 for comm in (self.ipc, self.ipc_act, self.ipc_w):
                     if comm is not None:
                         comm.reset_errors()

@@ -66,12 +66,19 @@ def run_trials(cands: Sequence[str], ops: TrialOps, *, forced: str = "auto", tim
                note: Callable[[str], None] = lambda m: None, clock: Optional[Callable[[], float]] = None,
                budget_s: float = 5.0) -> Tuple[List[float], List[float], set]:
     """Run every candidate from the same snapshot.  Returns (us per step, gradient deviation from the reference schedule,
-    names that are not eligible), the first two max-reduced over ranks and aligned with ``cands``."""
+    names that are not eligible), the first two max-reduced over ranks and aligned with ``cands``.  ``ops.expired_seen``: a
+    wait expired in some trial (agreed across ranks), also where a second try went well and nothing was dropped."""
     import time as _time
     clock = clock or _time.perf_counter
     times: List[float] = []
     grads: list = []
     broken: set = set()
+    ops.expired_seen = False
+
+    def expired_now() -> bool:
+        seen = ops.wait_expired()
+        ops.expired_seen = ops.expired_seen or seen
+        return seen
 
     def drop(c: str, why: str, restore: bool = False) -> None:
         note("%s: %s" % (c, why))
@@ -93,20 +100,21 @@ def run_trials(cands: Sequence[str], ops: TrialOps, *, forced: str = "auto", tim
             drop(c, "not eligible (graph capture failed on some rank)")
             continue
         grads.append(ops.first_step())
-        expired = c != "rccl" and ops.wait_expired()
+        expired = c != "rccl" and expired_now()
         if expired and c == REFERENCE:
             # nothing can be chosen without the reference's gradient, and ranks that time-share a GPU can miss the bound
             # once without anything being wrong: one more try from the snapshot
             note("%s: an in-kernel wait expired (2 s bound) in the first step; trying once more" % c)
             ops.restore()
             grads[-1] = ops.first_step()
-            expired = ops.wait_expired()
+            expired = expired_now()
         if expired:
             drop(c, "an in-kernel wait expired (2 s bound): not eligible", restore=True)
             continue
         if timed:
             t_us = ops.time_steps()
             if math.isinf(t_us):  # (agreed across ranks: TrialOps.time_steps stops at the first expired wait)
+                ops.expired_seen = True
                 drop(c, "an in-kernel wait expired during the timed steps (2 s bound): not eligible", restore=True)
                 continue
             times.append(t_us)
