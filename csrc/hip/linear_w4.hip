@@ -3,7 +3,7 @@
 // For single rows and small batches the weights' bytes are what the product costs (half a byte each, and 2 / G for the scales), so they
 // are laid out once as the matrix instruction wants them: a wave loads 16 outputs x 128 k as one contiguous KB.  Four
 // v_mfma_f32_16x16x32_bf16 take it: A = the weights, turned into bf16 two at a time by v_cvt_scalef32_pk_bf16_fp4 (0, 0.5 .. 6 are exact),
-// B = up to 16 rows of x.  With a single row 15 columns of B are idle, which costs nothing: the instruction is not what bounds the kernel,
+// B = 16 rows of x.  With a single row 15 columns of B are idle, which costs nothing: the instruction is not what bounds the kernel,
 // and unpacking to fp32 for vector FMAs would need three times the VALU work.  The group's scales are applied in fp32 to the
 // accumulator of the group (G = 32, 64, 128: 1, 2, 4 instructions).  16384 x 16384 take 28-29 us for 1 row (bf16, G = 64) and 16 (e4m3,
 // G = 128): 4.9 TB/s of weights, where a large copy reaches 5.1.
@@ -116,19 +116,22 @@ template <int NG> __device__ __forceinline__ uint32_t from_lane_of_four(uint32_t
   }
 }
 
-// GJ: matrix instructions (32 k each) that share a scale; R: tiles of 16 outputs a wave; PIECES: of x a lane, one for few rows
-template <int XT, int GJ, int R, int PIECES> __global__ __launch_bounds__(512) void linear_w4_kernel(const LinearW4Args a) {
+// GJ: matrix instructions (32 k each) that share a scale; R: tiles of 16 outputs a wave; C: tiles of 16 columns of B; PIECES: of x a lane,
+// one for few rows
+template <int XT, int GJ, int R, int C, int PIECES> __global__ __launch_bounds__(C == 1 ? 512 : 256) void linear_w4_kernel(const LinearW4Args a) {
   using T = typename XType<XT>::T;
-  constexpr int P = XType<XT>::P, MC = 16 / P, NG = 4 / GJ;
+  constexpr int P = XType<XT>::P, MC = C * 16 / P, NG = 4 / GJ;
   constexpr int E = 16 / sizeof(T), PER_ROW = 128 / E;  // elements of a piece, pieces of a row
-  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // a tile of x for each wave; at the end [waves][R][16 n][16 columns] sums
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // a tile of x for each wave; at the end [waves][R][16 n][C * 16 columns] sums
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, kb = lane >> 4, col = lane & 15;
   const int nt_all = (a.N + 15) / 16, kt_all = (a.K + 127) / 128, nt0 = blockIdx.x * R;
   const long m0 = (long)blockIdx.y * MC;
   const int rows = (int)min((long)MC, a.M - m0);  // of this pass
   const T* const x0 = static_cast<const T*>(a.x) + m0 * a.ldx;
-  uint16_t* const tile = reinterpret_cast<uint16_t*>(lds) + wave * 16 * PITCH;
-  const uint16_t* const column = tile + min(col, rows * P - 1) * PITCH + 8 * kb;  // (columns behind the last repeat it: not stored)
+  uint16_t* const tile = reinterpret_cast<uint16_t*>(lds) + wave * C * 16 * PITCH;
+  const uint16_t* column[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) column[c] = tile + min(16 * c + col, rows * P - 1) * PITCH + 8 * kb;  // (columns behind the last repeat it: not stored)
   const uint4* wq[R];
   const uint16_t* sc[R];
 #pragma unroll
@@ -137,9 +140,11 @@ template <int XT, int GJ, int R, int PIECES> __global__ __launch_bounds__(512) v
     wq[r] = static_cast<const uint4*>(a.wq) + nt * kt_all * 64 + lane;
     sc[r] = a.scales + (nt * kt_all * NG + col % NG) * 16 + 4 * kb;  // (the tile's groups are shared out over each four lanes)
   }
-  f32x4 acc[R];
+  f32x4 acc[R][C];
 #pragma unroll
-  for (int r = 0; r < R; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[r][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   struct Weights {
     uint4 w[R];
     uint2 s[R];
@@ -151,7 +156,7 @@ template <int XT, int GJ, int R, int PIECES> __global__ __launch_bounds__(512) v
       t.s[r] = *reinterpret_cast<const uint2*>(sc[r] + (long)kt * NG * 16);
     }
   };
-  auto multiply = [&](const Weights& t, const XPiece (&x)[PIECES]) {
+  auto put = [&](const XPiece (&x)[PIECES]) {  // a tile of x into LDS
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       const int c = i * 64 + lane;
@@ -160,27 +165,39 @@ template <int XT, int GJ, int R, int PIECES> __global__ __launch_bounds__(512) v
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (a wave's own tile: its LDS accesses are done in order)
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    bf16x8 b[4];
+  };
+  auto multiply = [&](const Weights& t) {  // with the tile of x that is in LDS
 #pragma unroll
-    for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const bf16x8*>(column + 32 * j);
+    for (int g = 0; g < NG; ++g) {
+      bf16x8 b[GJ][C];
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+      for (int j = 0; j < GJ; ++j)
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        f32x4 d = {0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < C; ++c) b[j][c] = *reinterpret_cast<const bf16x8*>(column[c] + 32 * (g * GJ + j));
 #pragma unroll
-        for (int j = g * GJ; j < (g + 1) * GJ; ++j)
-          d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e2m1_bf16(reinterpret_cast<const uint32_t*>(&t.w[r])[j]), b[j], d, 0, 0, 0);
+      for (int r = 0; r < R; ++r) {
+        f32x4 d[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) d[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < GJ; ++j) {
+          const bf16x8 w = e2m1_bf16(reinterpret_cast<const uint32_t*>(&t.w[r])[g * GJ + j]);
+#pragma unroll
+          for (int c = 0; c < C; ++c) d[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, b[j][c], d[c], 0, 0, 0);
+        }
         const uint2 q = make_uint2(from_lane_of_four<NG>(t.s[r].x, g), from_lane_of_four<NG>(t.s[r].y, g));
         const float s4[4] = {__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u), __uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u)};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[r][i] = fmaf(d[i], s4[i], acc[r][i]);
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[r][c][i] = fmaf(d[c][i], s4[i], acc[r][c][i]);
       }
+    }
+    __builtin_amdgcn_wave_barrier();
   };
   // Whole tiles of k; the next tile's loads are on their way while one is multiplied.
   const int whole = a.K / 128;
-  auto fetch = [&](Weights& t, XPiece (&x)[PIECES], int kt) {
-    load(t, kt);
+  auto fetch = [&](XPiece (&x)[PIECES], int kt) {
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       const int c = i * 64 + lane;
@@ -189,19 +206,24 @@ template <int XT, int GJ, int R, int PIECES> __global__ __launch_bounds__(512) v
   };
   if (wave < whole) {
     Weights t, t2;
-    XPiece x[PIECES], x2[PIECES];
-    fetch(t, x, wave);
+    XPiece x[PIECES];
+    fetch(x, wave);
+    load(t, wave);
     for (int kt = wave; kt < whole; kt += 2 * waves) {
       // (behind the end: this one again, not multiplied.  Without a branch, so that the compiler counts the loads that are still out and
       // waits for the older half alone: behind a branch it waits for all, 8.9 instead of 7.6 us for one row of 16384 by 2048 outputs)
-      fetch(t2, x2, kt + waves < whole ? kt + waves : kt);
+      const int second = kt + waves < whole ? kt + waves : kt, third = kt + 2 * waves < whole ? kt + 2 * waves : kt;
+      put(x);
+      fetch(x, second);
+      load(t2, second);
       __builtin_amdgcn_sched_barrier(0);
-      multiply(t, x);
-      __builtin_amdgcn_wave_barrier();
-      fetch(t, x, kt + 2 * waves < whole ? kt + 2 * waves : kt);
+      multiply(t);
+      if (second == kt) break;
+      put(x);
+      fetch(x, third);
+      load(t, third);
       __builtin_amdgcn_sched_barrier(0);
-      if (kt + waves < whole) multiply(t2, x2);
-      __builtin_amdgcn_wave_barrier();
+      multiply(t2);
     }
   }
   if (whole < kt_all && wave == whole % waves) {  // the rest of k: zeros behind it, nothing behind a row's end is read
@@ -213,14 +235,17 @@ template <int XT, int GJ, int R, int PIECES> __global__ __launch_bounds__(512) v
       const int c = i * 64 + lane;
       x[i] = last_piece(x0 + min(c / PER_ROW, rows - 1) * a.ldx, whole * 128 + c % PER_ROW * E, a.K);
     }
-    multiply(t, x);
+    put(x);
+    multiply(t);
   }
   __syncthreads();
   float* const part = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part[((wave * R + r) * 16 + 4 * kb + i) * 16 + col] = acc[r][i];
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[((wave * R + r) * 16 + 4 * kb + i) * (C * 16) + 16 * c + col] = acc[r][c][i];
   __syncthreads();
   for (int o = threadIdx.x; o < R * 16 * MC; o += blockDim.x) {
     const int n = o % (R * 16), mm = o / (R * 16);
@@ -230,7 +255,7 @@ template <int XT, int GJ, int R, int PIECES> __global__ __launch_bounds__(512) v
     float s = 0.f;
     for (int w = 0; w < waves; ++w)
 #pragma unroll
-      for (int p = 0; p < P; ++p) s += part[(w * R * 16 + n) * 16 + mm * P + p];
+      for (int p = 0; p < P; ++p) s += part[(w * R * 16 + n) * (C * 16) + mm * P + p];
     if (a.x_scale) s *= a.x_scale[m];
     if (a.bias) s += a.bias[out];
     if (a.relu) s = s < 0.f ? 0.f : s;  // (a NaN stays one)
@@ -240,28 +265,49 @@ template <int XT, int GJ, int R, int PIECES> __global__ __launch_bounds__(512) v
 }
 
 namespace {
-template <int XT, int GJ, int R> void go(const LinearW4Args& a, int passes, hipStream_t st) {
-  constexpr int ROW = 128 * sizeof(typename XType<XT>::T), MC = 16 / XType<XT>::P, MOST = (MC * ROW + 1023) / 1024;  // bytes of a tile's row; KB of a tile
-  // eight waves split k (4: 15.2 instead of 9.1 us for one row of 16384 by 2048 outputs; 16: 10.3, and even elsewhere)
-  const int nt = (a.N + 15) / 16, kt = (a.K + 127) / 128, waves = kt < 8 ? kt : 8;
+template <int XT, int GJ, int R, int C> void go(const LinearW4Args& a, int passes, hipStream_t st) {
+  constexpr int ROW = 128 * sizeof(typename XType<XT>::T), MC = C * 16 / XType<XT>::P, MOST = (MC * ROW + 1023) / 1024;  // bytes of a tile's row; KB of a tile
+  // eight waves split k (4: 15.2 instead of 9.1 us for one row of 16384 by 2048 outputs; 16: 10.3, and even elsewhere); four where each has
+  // more to do, and its registers and LDS are more (7: 17.7 instead of 15.6 us for 32 rows bf16, 4096 x 16384)
+  constexpr int most = C == 1 ? 8 : 4;
+  const int nt = (a.N + 15) / 16, kt = (a.K + 127) / 128, waves = kt < most ? kt : most;
   const dim3 grid((nt + R - 1) / R, passes);
-  static_assert(32 * PITCH >= R * 1024, "a wave's sums take the place of its tile of x");
-  const int lds = 32 * PITCH * waves;
-  if (a.M * ROW <= 1024) hipLaunchKernelGGL((linear_w4_kernel<XT, GJ, R, 1>), grid, dim3(64 * waves), lds, st, a);
-  else hipLaunchKernelGGL((linear_w4_kernel<XT, GJ, R, MOST>), grid, dim3(64 * waves), lds, st, a);
+  static_assert(32 * PITCH >= R * 1024, "a wave's sums take the place of its tiles of x");
+  const int lds = 32 * PITCH * C * waves;
+  if constexpr (C == 1) {
+    if (a.M * ROW <= 1024) {
+      hipLaunchKernelGGL((linear_w4_kernel<XT, GJ, R, C, 1>), grid, dim3(64 * waves), lds, st, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((linear_w4_kernel<XT, GJ, R, C, MOST>), grid, dim3(64 * waves), lds, st, a);
 }
-// More rows than the columns of B hold (16; fp32 5) take a pass over the weights for each such set, side by side in one launch (several
-// column tiles a wave were slower: 64 rows bf16, 4096 x 16384, 35.5 instead of 30.6 us).  A wave takes as many tiles of outputs as leave the
-// chip filled, because each tile of x is then loaded and turned less often.  Measured, us with 1 / 2 / 4 tiles, by tiles of outputs x passes:
-// 256 (16 rows bf16, 4096 x 4096) 4.8 / 6.0 / 8.7; 512 (1 row bf16, 8192 x 8192) 8.1 / 8.0 / 9.9, (5 rows fp32) 14.0 / 11.1 / 15.1; 750 (16 rows
-// bf16, 4096 x 12000) 9.8 / 10.5 / 9.9; 1024 (16 rows e4m3, 16384 x 16384) 39.1 / 31.6 / 28.9, (1 row bf16) 28.6 / 27.3 / 28.2.
+// How many tiles of outputs (R) and of 16 columns of B (C) a wave takes: as many as leave the chip filled, because a tile of x is then loaded
+// and turned less often (R), and a tile of weights loaded and unpacked less often (C).  Rows that the columns do not hold take another pass
+// over the weights, side by side in one launch.  us measured by tiles of outputs x passes:
+// - C = 1, R = 1 / 2 / 4: 256 (16 rows bf16, 4096 x 4096) 4.6 / 6.0 / 8.7; 512 (1 row bf16, 8192 x 8192) 8.1 / 8.0 / 9.9; 750 (16 rows bf16,
+//   4096 x 12000) 9.8 / 10.5 / 9.9; 1024 (16 rows e4m3, 16384 x 16384) 39.1 / 31.6 / 29.6.
+// - C = 2, R = 2 / 4, and the best of C = 1: 512 (10 rows fp32, 4096 x 8192) 12.9 / 17.9, 10.8; 750 (32 rows bf16, 4096 x 12000) 15.2 / 16.3, 14.3; 1024
+//   (32 rows bf16, 4096 x 16384) 15.5 / 15.6, 18.1, (6 rows fp32, 16384 x 16384) 54.4 / 46.7, 54.6, (128 rows bf16, 4096 x 4096) 15.1 / 16.3, 16.4;
+//   2048 (64 rows bf16, 4096 x 16384) 26.4 / 24.1, 31.9.
+// - C = 3, R = 2 / 4, and the best of C = 1: 375 (16 rows fp32, 4096 x 6000) 15.9 / 21.6, 16.1; 512 (the same, 8192 x 8192) 26.8 / 36.0, 29.4; 750 (4096 x
+//   12000) 22.5 / 22.0, 27.8; 1024 (4096 x 16384) 22.9 / 22.3, 35.0.  Only fp32 rows gain by it (48 rows bf16, 4096 x 8192: 13.0, 13.8), and C = 4 is
+//   slower than 2 for all but the largest products.
 template <int XT, int GJ> void with_tiles(const LinearW4Args& a, hipStream_t st) {
-  constexpr int MC = 16 / XType<XT>::P;
-  const int passes = (int)((a.M + MC - 1) / MC);
-  const long sets = (long)((a.N + 15) / 16) * passes;
-  if (sets >= 1024) go<XT, GJ, 4>(a, passes, st);
-  else if (sets >= 512) go<XT, GJ, 2>(a, passes, st);
-  else go<XT, GJ, 1>(a, passes, st);
+  const long nt = (a.N + 15) / 16;
+  auto passes = [&](int c) {
+    const long rows = c * 16 / XType<XT>::P;
+    return (a.M + rows - 1) / rows;
+  };
+  if constexpr (XT == X_F32) {
+    if (passes(3) < passes(2) && nt * passes(3) >= 512)
+      return nt * passes(3) >= 1024 ? go<XT, GJ, 4, 3>(a, (int)passes(3), st) : go<XT, GJ, 2, 3>(a, (int)passes(3), st);
+  }
+  if (passes(2) < passes(1) && nt * passes(2) >= 1024) return go<XT, GJ, 4, 2>(a, (int)passes(2), st);
+  const long sets = nt * passes(1);
+  if (sets >= 1024) go<XT, GJ, 4, 1>(a, (int)passes(1), st);
+  else if (sets >= 512) go<XT, GJ, 2, 1>(a, (int)passes(1), st);
+  else go<XT, GJ, 1, 1>(a, (int)passes(1), st);
 }
 template <int XT> void with_group(const LinearW4Args& a, hipStream_t st) {
   if (a.group == 32) with_tiles<XT, 1>(a, st);

@@ -59,6 +59,15 @@ def test_products(M, K, N, group, dtype):
     check(hip_ops.linear_w4(x, wq, scales, N, relu=True, x_scale=scale, out_dtype=B), x, scale, w, None, True)
 
 
+# two and three tiles of columns a wave (more rows than one tile holds, outputs or rows enough to fill the chip): fewer k than a tile, fewer
+# tiles of k than waves, a tail; all columns taken, a last pass of one row, an odd number of output tiles
+@pytest.mark.parametrize("dtype", [F, B, E])
+@pytest.mark.parametrize("M,K,N,group", [(16, 100, 8200, 32), (12, 300, 16390, 64), (6, 515, 16400, 128), (10, 1000, 16384, 32), (17, 64, 16385, 64),
+                                         (32, 777, 16390, 32), (1025, 129, 520, 32), (1030, 512, 500, 128), (257, 1001, 514, 64), (353, 260, 1030, 128)])
+def test_several_tiles_of_columns(M, K, N, group, dtype):
+    test_products(M, K, N, group, dtype)
+
+
 @pytest.mark.parametrize("dtype", [F, B, E])
 @pytest.mark.parametrize("K", [256, 257, 264])
 def test_strides_alignment_and_leading_dimensions(K, dtype):
