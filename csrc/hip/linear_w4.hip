@@ -65,7 +65,7 @@ template <typename T> __device__ __forceinline__ XPiece last_piece(const T* row,
 // few rows are read by up to 16 lanes each (and converted as often), and the load unit, not memory, is what bounds the kernel.
 // PITCH: 16 columns' parts of 16 bytes fall into all 64 banks.
 constexpr int PITCH = 128 + 8;
-template <int XT> __device__ __forceinline__ void store_columns(uint16_t* tile, int row, int k, const XPiece& x) {
+template <int XT, bool CHECKED> __device__ __forceinline__ void store_columns(uint16_t* tile, int row, int k, const XPiece& x, float& sum) {
   if constexpr (XT == X_BF16) {
     *reinterpret_cast<uint4*>(tile + row * PITCH + k) = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
   } else if constexpr (XT == X_E4M3) {
@@ -79,23 +79,28 @@ template <int XT> __device__ __forceinline__ void store_columns(uint16_t* tile, 
     to[0] = make_uint4(u[0], u[1], u[2], u[3]);
     to[1] = make_uint4(u[4], u[5], u[6], u[7]);
   } else {
-    // the upper 16 bits, those of the rest, and what is left: both differences are exact.  The first column takes a NaN or an infinity (a
-    // NaN made quiet, so that one whose bits all lie in the lower half survives); infinity less itself, a NaN, is none of the others' business.
+    // the upper 16 bits, those of the rest, and what is left: both differences are exact
     uint32_t part[3][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float v = __uint_as_float(x.w[i]);
-      const uint32_t bits = x.w[i], nan = v != v ? 0x00400000u : 0u;
-      float rest = v - __uint_as_float(bits & 0xffff0000u);
-      rest = rest == rest ? rest : 0.f;
-      part[0][i] = bits | nan;
+      float rest = v - __uint_as_float(x.w[i] & 0xffff0000u);
+      part[0][i] = x.w[i];
+      if constexpr (CHECKED) {
+        // the first column takes a NaN or an infinity (a NaN made quiet, so that one whose bits all lie in the lower half survives); infinity
+        // less itself, a NaN, is none of the others' business
+        part[0][i] |= v != v ? 0x00400000u : 0u;
+        rest = rest == rest ? rest : 0.f;
+      } else {
+        sum += rest;  // (of finite values: finite)
+      }
       part[1][i] = __float_as_uint(rest);
       part[2][i] = __float_as_uint(rest - __uint_as_float(part[1][i] & 0xffff0000u));
     }
 #pragma unroll
     for (int p = 0; p < 3; ++p)
       *reinterpret_cast<uint2*>(tile + (3 * row + p) * PITCH + k) =
-          make_uint2((part[p][0] >> 16) | (part[p][1] & 0xffff0000u), (part[p][2] >> 16) | (part[p][3] & 0xffff0000u));
+          make_uint2(__builtin_amdgcn_perm(part[p][1], part[p][0], 0x07060302u), __builtin_amdgcn_perm(part[p][3], part[p][2], 0x07060302u));
   }
 }
 __device__ __forceinline__ bf16x8 e2m1_bf16(uint32_t w) {  // eight codes, the low nibble of the low byte first
@@ -157,10 +162,18 @@ template <int XT, int GJ, int R, int C, int PIECES> __global__ __launch_bounds__
     }
   };
   auto put = [&](const XPiece (&x)[PIECES]) {  // a tile of x into LDS
+    float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
       const int c = i * 64 + lane;
-      store_columns<XT>(tile, min(c / PER_ROW, MC - 1), c % PER_ROW * E, x[i]);  // (rows behind the last hold it again)
+      store_columns<XT, false>(tile, min(c / PER_ROW, MC - 1), c % PER_ROW * E, x[i], sum);  // (rows behind the last hold it again)
+    }
+    if (XT == X_F32 && __any(sum != sum)) {  // a NaN or an infinity: once more
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) {
+        const int c = i * 64 + lane;
+        store_columns<XT, true>(tile, min(c / PER_ROW, MC - 1), c % PER_ROW * E, x[i], sum);
+      }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // (a wave's own tile: its LDS accesses are done in order)
     __builtin_amdgcn_wave_barrier();

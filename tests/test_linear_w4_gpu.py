@@ -59,13 +59,43 @@ def test_products(M, K, N, group, dtype):
     check(hip_ops.linear_w4(x, wq, scales, N, relu=True, x_scale=scale, out_dtype=B), x, scale, w, None, True)
 
 
-# two and three tiles of columns a wave (more rows than one tile holds, outputs or rows enough to fill the chip): fewer k than a tile, fewer
-# tiles of k than waves, a tail; all columns taken, a last pass of one row, an odd number of output tiles
+# two and three tiles of columns a wave (more rows than one tile holds, outputs or rows enough to fill the chip), each with one to four tiles of
+# outputs: fewer k than a tile, fewer tiles of k than waves, a tail; all columns taken, a last pass of one row, an odd number of output tiles
 @pytest.mark.parametrize("dtype", [F, B, E])
 @pytest.mark.parametrize("M,K,N,group", [(16, 100, 8200, 32), (12, 300, 16390, 64), (6, 515, 16400, 128), (10, 1000, 16384, 32), (17, 64, 16385, 64),
-                                         (32, 777, 16390, 32), (1025, 129, 520, 32), (1030, 512, 500, 128), (257, 1001, 514, 64), (353, 260, 1030, 128)])
+                                         (32, 777, 16390, 32), (1025, 129, 520, 32), (1030, 512, 500, 128), (257, 1001, 514, 64), (353, 260, 1030, 128), (12300, 130, 9, 32),
+                                         (16, 140, 11000, 64), (32, 8300, 11000, 32), (7, 200, 9700, 32), (40, 100, 4700, 64), (5000, 70, 20, 64),
+                                         (17, 128, 12352, 64), (17, 130, 18490, 32), (33, 100, 13700, 128), (11, 200, 8190, 64), (21, 390, 13700, 32), (3000, 128, 32, 128)])
 def test_several_tiles_of_columns(M, K, N, group, dtype):
     test_products(M, K, N, group, dtype)
+
+
+# fp32 rows are cut into three parts: a NaN or an infinity reaches its own row alone, in a whole tile of k and in the last one, and a NaN whose
+# bits all lie in the lower half stays one; the largest and the smallest finite values are summed exactly
+@pytest.mark.parametrize("M,K,N", [(3, 300, 40), (16, 300, 8200), (6, 300, 16400)])
+def test_fp32_values_at_the_ends_of_the_range(M, K, N):
+    from distributed_tensorflow_amd.ops import hip_ops
+    wq, scales, w = _weights(K, N, 32)
+    x, _ = _rows(M, K, F)
+    clean = hip_ops.linear_w4(x, wq, scales, N)
+    used = w.abs().sum(1) != 0
+    assert bool(used[7]) and bool(used[290])
+    for k in (7, 290):
+        for bits in (0x7f800000, 0xff800000, 0x7f800001, 0x7fc00000):
+            z = x.clone()
+            z.view(torch.int32)[1, k] = bits - (1 << 32) if bits >> 31 else bits
+            y = hip_ops.linear_w4(z, wq, scales, N)
+            hit = w[k] != 0
+            assert bool(y[1, hit].isfinite().logical_not().all())
+            assert torch.equal(y[1].isnan()[hit], torch.full_like(hit, bits & 0x7fffff != 0)[hit])
+            rest = torch.arange(M, device="cuda") != 1
+            assert torch.equal(y[rest], clean[rest])
+    for v in (torch.finfo(F).max / 2 ** 20, 2.0 ** -100):
+        z = torch.zeros_like(x)
+        z[:, 7] = v
+        y = hip_ops.linear_w4(z, wq, scales, N).double()
+        want = z.double() @ w
+        assert bool(((y - want).abs() <= 8 * U * want.abs()).all())
 
 
 @pytest.mark.parametrize("dtype", [F, B, E])
