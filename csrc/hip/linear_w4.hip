@@ -295,32 +295,48 @@ template <int XT, int GJ, int R, int C> void go(const LinearW4Args& a, int passe
   }
   hipLaunchKernelGGL((linear_w4_kernel<XT, GJ, R, C, MOST>), grid, dim3(64 * waves), lds, st, a);
 }
-// How many tiles of outputs (R) and of 16 columns of B (C) a wave takes: as many as leave the chip filled, because a tile of x is then loaded
-// and turned less often (R), and a tile of weights loaded and unpacked less often (C).  Rows that the columns do not hold take another pass
-// over the weights, side by side in one launch.  us measured by tiles of outputs x passes:
-// - C = 1, R = 1 / 2 / 4: 256 (16 rows bf16, 4096 x 4096) 4.6 / 6.0 / 8.7; 512 (1 row bf16, 8192 x 8192) 8.1 / 8.0 / 9.9; 750 (16 rows bf16,
-//   4096 x 12000) 9.8 / 10.5 / 9.9; 1024 (16 rows e4m3, 16384 x 16384) 39.1 / 31.6 / 29.6.
-// - C = 2, R = 2 / 4, and the best of C = 1: 512 (10 rows fp32, 4096 x 8192) 12.9 / 17.9, 10.8; 750 (32 rows bf16, 4096 x 12000) 15.2 / 16.3, 14.3; 1024
-//   (32 rows bf16, 4096 x 16384) 15.5 / 15.6, 18.1, (6 rows fp32, 16384 x 16384) 54.4 / 46.7, 54.6, (128 rows bf16, 4096 x 4096) 15.1 / 16.3, 16.4;
-//   2048 (64 rows bf16, 4096 x 16384) 26.4 / 24.1, 31.9.
-// - C = 3, R = 2 / 4, and the best of C = 1: 375 (16 rows fp32, 4096 x 6000) 15.9 / 21.6, 16.1; 512 (the same, 8192 x 8192) 26.8 / 36.0, 29.4; 750 (4096 x
-//   12000) 22.5 / 22.0, 27.8; 1024 (4096 x 16384) 22.9 / 22.3, 35.0.  Only fp32 rows gain by it (48 rows bf16, 4096 x 8192: 13.0, 13.8), and C = 4 is
-//   slower than 2 for all but the largest products.
+// How many tiles of outputs (R) and of 16 columns of B (C) a wave takes.  More of the first: a tile of x is loaded and turned less often; of
+// the second: a tile of weights is loaded and unpacked less often.  Rows that the columns do not hold take another pass over the weights, side by
+// side in one launch.  What decides is how the workgroups come out on the 256 CUs, so the time is estimated as
+//   first[C][R] * (1 + more * (rounds - 1)),   rounds = workgroups / 256, upwards
+// where first is what one round takes (us measured for k = 4096) and another one adds less, because two workgroups share a CU by then; less still
+// for short k, where much of a workgroup's time is waiting at its ends.  Measured, us (chosen: *):
+//   C = 1, R = 1 / 2 / 3 / 4     3 rows fp32, 5000 x 4160 (260 tiles of outputs)  8.8 / 8.5* / 9.8 / 11.7    1 row bf16, 16384 x 9600 (600)  17.0 / 19.5 / 14.9* / 17.2
+//                                16 rows e4m3, 5000 x 12288 (768)  10.6 / 11.8 / 10.0* / 11.4                the same, 16384 x 16384  39.1 / 31.6 / - / 29.6*
+//   C = 1, C = 2, R = 2 / 3 / 4  32 rows bf16, 4096 x 16384  17.5, 15.3* / 18.4 / 16.6                       10 rows fp32, 16384 x 16384  60.4, 59.9 / - / 46.4*
+//   C = 1, C = 3, R = 2 / 3 / 4  16 rows fp32, 4096 x 8192  17.3, 14.2* / 16.5 / 20.2                        the same, 16384 x 16384  98, 66 / 71 / 59*
+// Three column tiles help fp32 rows alone (48 rows bf16, 4096 x 8192: 13.0 instead of 13.8), four are slower than two for all but the largest.
 template <int XT, int GJ> void with_tiles(const LinearW4Args& a, hipStream_t st) {
+  static const float first[3][4] = {{4.7f, 6.1f, 8.1f, 9.1f}, {0.f, 10.6f, 13.2f, 16.f}, {0.f, 13.6f, 16.3f, 19.7f}};
+  static const float more1[4] = {.5f, .62f, .62f, 1.f};
+  constexpr int MOST_C = XT == X_F32 ? 3 : 2;
   const long nt = (a.N + 15) / 16;
-  auto passes = [&](int c) {
-    const long rows = c * 16 / XType<XT>::P;
-    return (a.M + rows - 1) / rows;
-  };
-  if constexpr (XT == X_F32) {
-    if (passes(3) < passes(2) && nt * passes(3) >= 512)
-      return nt * passes(3) >= 1024 ? go<XT, GJ, 4, 3>(a, (int)passes(3), st) : go<XT, GJ, 2, 3>(a, (int)passes(3), st);
+  const bool few = a.M * 128 * (long)sizeof(typename XType<XT>::T) <= 1024;  // (x takes a wave one load a tile: 2 rows bf16, 2866 x 5194: 4.5 instead of 4.9 us)
+  float least = 0.f;
+  int best = -1, passes = 0;
+  for (int c = 1; c <= MOST_C; ++c)
+    for (int r = c == 1 ? 1 : 2; r <= 4; ++r) {  // (one tile of outputs with several of columns comes out best for next to nothing)
+      const long rows = c * 16 / XType<XT>::P, p = (a.M + rows - 1) / rows, rounds = ((nt + r - 1) / r * p + 255) / 256;
+      const float more = c == 1 && r == 1 && rounds == 2 && few ? .25f : c == 1 ? more1[r - 1] : a.K < 8192 ? .4f : .6f;
+      const float t = first[c - 1][r - 1] * (1.f + more * (float)(rounds - 1));
+      if (best < 0 || t < least) least = t, best = 4 * c + r - 5, passes = (int)p;
+    }
+  switch (best) {
+    case 0: return go<XT, GJ, 1, 1>(a, passes, st);
+    case 1: return go<XT, GJ, 2, 1>(a, passes, st);
+    case 2: return go<XT, GJ, 3, 1>(a, passes, st);
+    case 3: return go<XT, GJ, 4, 1>(a, passes, st);
+    case 5: return go<XT, GJ, 2, 2>(a, passes, st);
+    case 6: return go<XT, GJ, 3, 2>(a, passes, st);
+    case 7: return go<XT, GJ, 4, 2>(a, passes, st);
   }
-  if (passes(2) < passes(1) && nt * passes(2) >= 1024) return go<XT, GJ, 4, 2>(a, (int)passes(2), st);
-  const long sets = nt * passes(1);
-  if (sets >= 1024) go<XT, GJ, 4, 1>(a, (int)passes(1), st);
-  else if (sets >= 512) go<XT, GJ, 2, 1>(a, (int)passes(1), st);
-  else go<XT, GJ, 1, 1>(a, (int)passes(1), st);
+  if constexpr (MOST_C == 3) {
+    switch (best) {
+      case 9: return go<XT, GJ, 2, 3>(a, passes, st);
+      case 10: return go<XT, GJ, 3, 3>(a, passes, st);
+      case 11: return go<XT, GJ, 4, 3>(a, passes, st);
+    }
+  }
 }
 template <int XT> void with_group(const LinearW4Args& a, hipStream_t st) {
   if (a.group == 32) with_tiles<XT, 1>(a, st);
