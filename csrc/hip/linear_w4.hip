@@ -123,7 +123,7 @@ template <int NG> __device__ __forceinline__ uint32_t from_lane_of_four(uint32_t
 
 // GJ: matrix instructions (32 k each) that share a scale; R: tiles of 16 outputs a wave; C: tiles of 16 columns of B; PIECES: of x a lane,
 // one for few rows
-template <int XT, int GJ, int R, int C, int PIECES> __global__ __launch_bounds__(C == 1 ? 512 : 256) void linear_w4_kernel(const LinearW4Args a) {
+template <int XT, int GJ, int R, int C, int PIECES> __global__ __launch_bounds__(C > 1 ? 256 : R > 1 ? 512 : 768) void linear_w4_kernel(const LinearW4Args a) {
   using T = typename XType<XT>::T;
   constexpr int P = XType<XT>::P, MC = C * 16 / P, NG = 4 / GJ;
   constexpr int E = 16 / sizeof(T), PER_ROW = 128 / E;  // elements of a piece, pieces of a row
@@ -280,11 +280,12 @@ template <int XT, int GJ, int R, int C, int PIECES> __global__ __launch_bounds__
 namespace {
 template <int XT, int GJ, int R, int C> void go(const LinearW4Args& a, int passes, hipStream_t st) {
   constexpr int ROW = 128 * sizeof(typename XType<XT>::T), MC = C * 16 / XType<XT>::P, MOST = (MC * ROW + 1023) / 1024;  // bytes of a tile's row; KB of a tile
-  // eight waves split k (4: 15.2 instead of 9.1 us for one row of 16384 by 2048 outputs; 16: 10.3, and even elsewhere); four where each has
-  // more to do, and its registers and LDS are more (7: 17.7 instead of 15.6 us for 32 rows bf16, 4096 x 16384)
-  constexpr int most = C == 1 ? 8 : 4;
-  const int nt = (a.N + 15) / 16, kt = (a.K + 127) / 128, waves = kt < most ? kt : most;
+  // eight waves split k (4: 11.1 instead of 7.5 us for one row of 16384 by 2048 outputs), twelve where k is long and the CUs have one workgroup each
+  // at most (6.5; 15: 6.6; with 4096 k 3.5 instead of 3.4).  Four where each has more to do, and its registers and LDS are more (7: 17.7 instead
+  // of 15.6 us for 32 rows bf16, 4096 x 16384)
+  const int nt = (a.N + 15) / 16, kt = (a.K + 127) / 128;
   const dim3 grid((nt + R - 1) / R, passes);
+  const int most = C > 1 ? 4 : R == 1 && kt >= 64 && (long)nt * passes <= 256 ? 12 : 8, waves = kt < most ? kt : most;
   static_assert(32 * PITCH >= R * 1024, "a wave's sums take the place of its tiles of x");
   const int lds = 32 * PITCH * C * waves;
   if constexpr (C == 1) {

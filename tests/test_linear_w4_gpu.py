@@ -60,12 +60,13 @@ def test_products(M, K, N, group, dtype):
 
 
 # two and three tiles of columns a wave (more rows than one tile holds, outputs or rows enough to fill the chip), each with one to four tiles of
-# outputs: fewer k than a tile, fewer tiles of k than waves, a tail; all columns taken, a last pass of one row, an odd number of output tiles
+# outputs; twelve waves for a long k: fewer k than a tile, fewer tiles of k than waves, a tail; all columns taken, a last pass of one row, an odd number of output tiles
 @pytest.mark.parametrize("dtype", [F, B, E])
 @pytest.mark.parametrize("M,K,N,group", [(16, 100, 8200, 32), (12, 300, 16390, 64), (6, 515, 16400, 128), (10, 1000, 16384, 32), (17, 64, 16385, 64),
                                          (32, 777, 16390, 32), (1025, 129, 520, 32), (1030, 512, 500, 128), (257, 1001, 514, 64), (353, 260, 1030, 128), (12300, 130, 9, 32),
                                          (16, 140, 11000, 64), (32, 8300, 11000, 32), (7, 200, 9700, 32), (40, 100, 4700, 64), (5000, 70, 20, 64),
-                                         (17, 128, 12352, 64), (17, 130, 18490, 32), (33, 100, 13700, 128), (11, 200, 8190, 64), (21, 390, 13700, 32), (3000, 128, 32, 128)])
+                                         (17, 128, 12352, 64), (17, 130, 18490, 32), (33, 100, 13700, 128), (11, 200, 8190, 64), (21, 390, 13700, 32), (3000, 128, 32, 128),
+                                         (3, 8100, 100, 64), (16, 9001, 40, 128), (37, 16384, 17, 32)])
 def test_several_tiles_of_columns(M, K, N, group, dtype):
     test_products(M, K, N, group, dtype)
 
