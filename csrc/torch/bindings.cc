@@ -7,6 +7,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -27,6 +28,11 @@ struct NativeError : std::runtime_error {  // native.NativeError on the Python s
 };
 void check(int rc, const char* what) {
   if (rc != 0) throw NativeError(c10::str(what, " failed with code ", rc, rc == -22 ? " (shape/alignment precondition violated)" : ""));
+}
+// A node that raises in a backward pass towards any of the operands.  (Its edges lead to them: one that hung from a leaf of its own would not
+// be visited by a gradient with respect to them alone.)
+template <typename... Operands> std::shared_ptr<torch::autograd::Node> refusal(const char* message, const Operands&... operands) {
+  return std::make_shared<torch::autograd::Error>(message, torch::autograd::collect_next_edges(operands...));
 }
 bool is_rows(const Tensor& t) {
   return t.is_cuda() && t.layout() == at::kStrided && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) && t.dim() >= 1;
@@ -178,12 +184,13 @@ struct RMSNormFunction : torch::autograd::Function<RMSNormFunction> {
       if (need_w) dw = at::zeros(w.sizes(), w.options());
     }
     torch::autograd::variable_list out{need_x ? dx : Tensor(), dw, need_r ? dx : Tensor(), Tensor()};
-    bool twice = at::GradMode::is_enabled() && ((dy.defined() && dy.requires_grad()) || (dh.defined() && dh.requires_grad()));
-    if (twice) {  // the kernels record nothing: a second derivative through them would be silently wrong
-      auto refuse = std::make_shared<torch::autograd::DelayedError>("rms_norm is differentiable once", (int)out.size());
+    // Under create_graph: the kernels record nothing, so that a second derivative through them would be silently wrong.  dx and dw depend on
+    // x, the residual and dy (dx on w and dh too, but it is asked for only where x or the residual requires a gradient).  h's own
+    // gradient is dh itself, whose graph goes on.
+    if (dy.defined() && at::GradMode::is_enabled() && (dy.requires_grad() || x.requires_grad() || (residual && residual->requires_grad()))) {
+      auto refuse = refusal("rms_norm is differentiable once", dy, dh, x, w, residual);
       for (auto& t : out)
-        if (t.defined()) t = t.detach().requires_grad_();
-      return (*refuse)(std::move(out));
+        if (t.defined()) torch::autograd::set_history(t = t.detach(), refuse);
     }
     return out;
   }

@@ -256,3 +256,46 @@ def test_refusals():
                 lambda: hip_ops.rms_norm_backward(x, x, torch.ones(4, device="cuda"), w, dh=x.to(B))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("residual", [False, True])
+def test_second_derivatives_are_refused_for_constant_incoming_gradients_too(residual):
+    """dx and dw depend on x, w and the residual also where dy does not require a gradient: y.sum(), or fixed grad_outputs."""
+    from distributed_tensorflow_amd.ops import autograd
+    gen, x, res, w = _inputs(7, 64, F, residual)
+    leaves = [t.requires_grad_() for t in (x, w, res) if t is not None]
+    dy = _rand(gen, 7, 64)
+
+    def grads(inputs):
+        y = autograd.rms_norm(x, w, res)
+        return torch.autograd.grad(y[0] if residual else y, inputs, dy, create_graph=True)
+
+    for leaf in leaves:
+        g, = grads([leaf])
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            (g.sum() + leaf.sum()).backward()
+    for g in grads(leaves):
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(g.sum(), leaves, allow_unused=True)
+    y = autograd.rms_norm(x, w, res)
+    g, = torch.autograd.grad((y[0] if residual else y).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (g * g).sum().backward()
+
+
+def test_what_has_a_second_derivative_or_none_is_not_refused():
+    from distributed_tensorflow_amd.ops import autograd
+    gen, x, res, w = _inputs(7, 64, F, True)
+    a = _rand(gen, 7, 64)
+    # dw of constant rows and a constant dy depends on nothing that requires a gradient
+    w.requires_grad_()
+    dw, = torch.autograd.grad(autograd.rms_norm(x, w), w, a, create_graph=True)
+    assert not dw.requires_grad and torch.equal(dw, torch.autograd.grad(autograd.rms_norm(x, w), w, a)[0])
+    # h = x + residual is linear: its gradient is dh itself, and dh's own graph goes on
+    x.requires_grad_()
+    a.requires_grad_()
+    _, h = autograd.rms_norm(x, w, res)
+    g, = torch.autograd.grad((h * a * a).sum(), x, create_graph=True)
+    assert torch.equal(g, a * a)
+    g.sum().backward()
+    assert torch.equal(a.grad, 2 * a.detach())
