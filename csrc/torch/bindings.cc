@@ -203,8 +203,8 @@ py::object rms_norm(const Tensor& x, const Tensor& w, const OptTensor& residual,
 
 // ------------------------------------------------------------------------------------------------ products with 4-bit weights
 constexpr int64_t W4_MAX_ROWS = 65535 * 5;
-Tensor linear_w4(const Tensor& x, const Tensor& wq, const Tensor& scales, int64_t N, const OptTensor& bias, bool relu, const OptTensor& x_scale,
-                 bool out_bf16) {
+Tensor w4_product(const Tensor& x, const Tensor& wq, const Tensor& scales, int64_t N, const OptTensor& bias, bool relu, const OptTensor& x_scale,
+                  bool out_bf16) {
   const at::NoGradGuard no_grad;
   TORCH_CHECK_VALUE(wq.scalar_type() == at::kByte && wq.dim() == 4 && wq.size(2) == 64 && wq.size(3) == 16 && wq.is_contiguous() && wq.numel() > 0 &&
                         scales.scalar_type() == at::kBFloat16 && scales.dim() == 3 && scales.is_contiguous() && scales.size(0) == wq.size(0) &&
@@ -247,6 +247,13 @@ Tensor linear_w4(const Tensor& x, const Tensor& wq, const Tensor& scales, int64_
   a.relu = relu;
   a.out_bf16 = out_bf16;
   check(dtf_linear_w4(&a, stream_of(x)), "linear_w4");
+  return y;
+}
+Tensor linear_w4(const Tensor& x, const Tensor& wq, const Tensor& scales, int64_t N, const OptTensor& bias, bool relu, const OptTensor& x_scale,
+                 bool out_bf16) {
+  const Tensor y = w4_product(x, wq, scales, N, bias, relu, x_scale, out_bf16);
+  if (torch::autograd::compute_requires_grad(x, scales, bias, x_scale))
+    torch::autograd::set_history(y, refusal("linear_w4 is for inference: it has no backward pass", x, scales, bias, x_scale));
   return y;
 }
 

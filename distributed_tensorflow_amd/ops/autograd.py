@@ -272,7 +272,8 @@ class Linear(nn.Module):
 
 
 class LinearW4(nn.Module):
-    """A trained ``Linear`` with 4-bit weights, for inference (``hip_ops.linear_w4``): ``LinearW4.from_linear(layer, group=64)``."""
+    """A trained ``Linear`` with 4-bit weights, for inference (``hip_ops.linear_w4``; a backward pass through it raises):
+    ``LinearW4.from_linear(layer, group=64)``."""
 
     def __init__(self, in_features: int, out_features: int, relu: bool = False, group: int = 64):
         super().__init__()

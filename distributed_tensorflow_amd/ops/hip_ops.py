@@ -415,7 +415,8 @@ def linear_w4(x: torch.Tensor, wq: torch.Tensor, scales: torch.Tensor, out_featu
 
     ``x[..., K]`` fp32 (not rounded), bf16, or e4m3 with ``x_scale`` (fp32, one a row; as ``rms_norm_e4m3`` gives them; optional for
     the other types); any stride between rows.  ``bias`` fp32 ``[out_features]``; the result fp32 or bf16 ``[..., out_features]``.  Sums are fp32.
-    More rows than 16 (fp32: 5), or 32 (fp32: 16) where the outputs are many enough, read the weights again."""
+    More rows than 16 (fp32: 5), or 32 (fp32: 16) where the outputs are many enough, read the weights again.  Where an operand requires a
+    gradient the result does too, and its backward pass raises: there is none."""
     if out_dtype not in (torch.float32, torch.bfloat16):
         raise ValueError("out_dtype is float32 or bfloat16 (got %s)" % (out_dtype,))
     return native.ext().linear_w4(x, wq, scales, out_features, bias, relu, x_scale, out_dtype == torch.bfloat16)

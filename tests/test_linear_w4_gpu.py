@@ -226,3 +226,31 @@ def test_empty_batches_and_refusals():
                 lambda: hip_ops.linear_w4(x[:1].expand(65535 * 5 + 1, 64), wq, scales, 32)):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("which", ["x", "bias", "x_scale"])
+def test_operands_that_require_a_gradient_make_the_backward_pass_raise(which):
+    """The values are those of any call; a loss that goes through the layer is refused instead of losing this branch's gradient."""
+    from distributed_tensorflow_amd.ops import autograd, hip_ops
+    wq, scales, w = _weights(200, 40, 64)
+    x, _ = _rows(3, 200, F)
+    ops = {"x": x, "bias": torch.ones(40, device="cuda"), "x_scale": torch.ones(3, device="cuda")}
+    want = hip_ops.linear_w4(ops["x"], wq, scales, 40, bias=ops["bias"], x_scale=ops["x_scale"])
+    leaf = ops[which].requires_grad_()
+    run = lambda: hip_ops.linear_w4(ops["x"], wq, scales, 40, bias=ops["bias"], x_scale=ops["x_scale"])  # noqa: E731
+    y = run()
+    assert torch.equal(y.detach(), want) and y.requires_grad
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        (y.sum() + leaf.sum()).backward()
+    assert leaf.grad is None
+    with torch.no_grad():
+        assert not run().requires_grad
+    # a gradient that does not go through the layer is taken as ever
+    other = torch.ones(3, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad((run().sum(1) * other).sum(), other)
+    assert torch.equal(g, want.sum(1))
+    if which == "x":  # the layer in the middle of a model that is trained
+        first, last = autograd.Linear(200, 200).cuda(), autograd.LinearW4.from_linear(autograd.Linear(200, 40).cuda())
+        hidden = first(x.detach())
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            (last(hidden).sum() + hidden.sum()).backward()
