@@ -34,6 +34,10 @@ void check(int rc, const char* what) {
 template <typename... Operands> std::shared_ptr<torch::autograd::Node> refusal(const char* message, const Operands&... operands) {
   return std::make_shared<torch::autograd::Error>(message, torch::autograd::collect_next_edges(operands...));
 }
+template <typename F> auto without_grad(F f) {
+  const at::NoGradGuard no_grad;
+  return f();
+}
 bool is_rows(const Tensor& t) {
   return t.is_cuda() && t.layout() == at::kStrided && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) && t.dim() >= 1;
 }
@@ -101,14 +105,27 @@ std::tuple<Tensor, Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& w
   }
   return {y, side, h};
 }
+// The results record no backward pass: one through them raises where `operands` require a gradient (h without a residual is x, whose gradient is
+// its own)
+template <typename... Operands>
+void refuse_backward(const std::tuple<Tensor, Tensor, Tensor>& out, const OptTensor& residual, const char* message, const Operands&... operands) {
+  if (!torch::autograd::compute_requires_grad(operands...)) return;
+  const auto fn = refusal(message, operands...);
+  torch::autograd::set_history(std::get<0>(out), fn);
+  torch::autograd::set_history(std::get<1>(out), fn);
+  if (residual) torch::autograd::set_history(std::get<2>(out), fn);
+}
 std::tuple<Tensor, Tensor, Tensor> rms_norm_forward(const Tensor& x, const Tensor& w, const OptTensor& residual, double eps) {
-  const at::NoGradGuard no_grad;
-  auto [y, rstd, h] = norm_forward(x, w, residual, eps, false);
+  const auto out = without_grad([&] { return norm_forward(x, w, residual, eps, false); });
+  // (not the weight: a layer's parameter is passed as it is by those who call rms_norm_backward themselves)
+  refuse_backward(out, residual, "rms_norm_forward has no backward pass of its own: autograd.rms_norm has", x, residual);
+  const auto& [y, rstd, h] = out;
   return {y, h, rstd};
 }
 std::tuple<Tensor, Tensor, Tensor> rms_norm_e4m3(const Tensor& x, const Tensor& w, const OptTensor& residual, double eps) {
-  const at::NoGradGuard no_grad;
-  return norm_forward(x, w, residual, eps, true);
+  const auto out = without_grad([&] { return norm_forward(x, w, residual, eps, true); });
+  refuse_backward(out, residual, "rms_norm_e4m3 is for inference: it has no backward pass", x, w, residual);
+  return out;
 }
 
 std::tuple<Tensor, OptTensor> rms_norm_backward(const Tensor& dy, const Tensor& x, const Tensor& rstd, const Tensor& w, const OptTensor& residual,

@@ -330,7 +330,8 @@ def rms_norm_forward(x: torch.Tensor, weight: torch.Tensor, residual: Optional[t
 
     ``x``, ``residual``: fp32 or bf16 rows of one type, any stride between rows; ``weight`` fp32.  ``h`` (``x`` itself without a
     residual) is rounded to that type, ``y`` comes from the unrounded sum; ``rstd`` (fp32, one a row) is for ``rms_norm_backward``.
-    Squares are summed in fp32: a row with magnitudes above 1e19 gives zeros."""
+    Squares are summed in fp32: a row with magnitudes above 1e19 gives zeros.  Nothing is recorded for autograd (``autograd.rms_norm`` is):
+    where ``x`` or ``residual`` requires a gradient a backward pass through the results raises; the weight is taken as a value."""
     return native.ext().rms_norm_forward(x, weight, residual, eps)
 
 
@@ -338,14 +339,15 @@ def rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torc
                   ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The same with an output in 8 bits, for inference: ``(q, scale, h)``, ``y ~ q * scale``; ``q`` e4m3 and ``scale`` fp32, one a
     row: its largest magnitude / 448.  A row of zeros has the scale 0, one that holds a NaN the scale NaN; a row whose largest magnitude is
-    below 2^-100 is scaled as if that were it."""
+    below 2^-100 is scaled as if that were it.  Where an operand requires a gradient a backward pass through the results raises: there is
+    none."""
     return native.ext().rms_norm_e4m3(x, weight, residual, eps)
 
 
 def rms_norm_backward(dy: torch.Tensor, x: torch.Tensor, rstd: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
                       dh: Optional[torch.Tensor] = None, need_dw: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``(dx, dw)`` of ``rms_norm_forward``; ``dx`` is the residual's gradient too.  ``dh``: the gradient that ``h`` has from elsewhere.
-    ``dw`` is summed in a fixed order: the same bits on every run."""
+    ``dw`` is summed in a fixed order: the same bits on every run.  Nothing is recorded: the results require no gradient."""
     return native.ext().rms_norm_backward(dy, x, rstd, weight, residual, dh, need_dw)
 
 

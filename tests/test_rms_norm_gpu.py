@@ -299,3 +299,24 @@ def test_what_has_a_second_derivative_or_none_is_not_refused():
     assert torch.equal(g, a * a)
     g.sum().backward()
     assert torch.equal(a.grad, 2 * a.detach())
+
+
+def test_the_forms_without_a_backward_pass_refuse_one():
+    """x or the residual requires a gradient: the values are those of any call, the backward pass raises instead of dropping it."""
+    from distributed_tensorflow_amd.ops import autograd, hip_ops
+    gen, x, res, w = _inputs(5, 200, B, True)
+    want8, want = hip_ops.rms_norm_e4m3(x, w, res), hip_ops.rms_norm_forward(x, w, res)
+    for name in ("x", "res"):
+        z, r = (x.clone().requires_grad_(), res) if name == "x" else (x, res.clone().requires_grad_())
+        for got, ref in ((hip_ops.rms_norm_e4m3(z, w, r), want8), (hip_ops.rms_norm_forward(z, w, r), want)):
+            for a, b in zip(got, ref):
+                assert torch.equal(a.detach().view(torch.uint8), b.view(torch.uint8))
+                with pytest.raises(RuntimeError, match="no backward pass"):
+                    a.float().sum().backward()
+        with torch.no_grad():
+            assert not any(t.requires_grad for t in hip_ops.rms_norm_e4m3(z, w, r) + hip_ops.rms_norm_forward(z, w, r))
+    z = x.clone().requires_grad_()
+    q, scale, h = hip_ops.rms_norm_e4m3(z, w)
+    assert h is z and q.requires_grad  # (without a residual h is x, whose gradient is its own)
+    layer = autograd.RMSNorm(200).cuda()
+    assert hip_ops.rms_norm_e4m3(x, layer.weight)[0].requires_grad  # (its weight has no gradient here either)
