@@ -307,35 +307,41 @@ template <int XT, int GJ, int R, int C> void go(const LinearW4Args& a, int passe
 //   C = 1, C = 2, R = 2 / 3 / 4  32 rows bf16, 4096 x 16384  17.5, 15.3* / 18.4 / 16.6                       10 rows fp32, 16384 x 16384  60.4, 59.9 / - / 46.4*
 //   C = 1, C = 3, R = 2 / 3 / 4  16 rows fp32, 4096 x 8192  17.3, 14.2* / 16.5 / 20.2                        the same, 16384 x 16384  98, 66 / 71 / 59*
 // Three column tiles help fp32 rows alone (48 rows bf16, 4096 x 8192: 13.0 instead of 13.8), four are slower than two for all but the largest.
-template <int XT, int GJ> void with_tiles(const LinearW4Args& a, hipStream_t st) {
+// A tile of columns that would hold no row is never worth it, whatever the estimate says (1 row bf16, 4096 x 262144: 150 us with one, 105 without).
+struct Tiles { int r, c, passes; };
+Tiles pick_tiles(long rows, int outputs, int k, int xtype) {
   static const float first[3][4] = {{4.7f, 6.1f, 8.1f, 9.1f}, {0.f, 10.6f, 13.2f, 16.f}, {0.f, 13.6f, 16.3f, 19.7f}};
   static const float more1[4] = {.5f, .62f, .62f, 1.f};
-  constexpr int MOST_C = XT == X_F32 ? 3 : 2;
-  const long nt = (a.N + 15) / 16;
-  const bool few = a.M * 128 * (long)sizeof(typename XType<XT>::T) <= 1024;  // (x takes a wave one load a tile: 2 rows bf16, 2866 x 5194: 4.5 instead of 4.9 us)
+  const int most_c = xtype == X_F32 ? 3 : 2, parts = xtype == X_F32 ? 3 : 1, size = xtype == X_F32 ? 4 : xtype == X_BF16 ? 2 : 1;
+  const long nt = ((long)outputs + 15) / 16;
+  const bool few = rows * 128 * size <= 1024;  // (x takes a wave one load a tile: 2 rows bf16, 2866 x 5194: 4.5 instead of 4.9 us)
   float least = 0.f;
-  int best = -1, passes = 0;
-  for (int c = 1; c <= MOST_C; ++c)
+  Tiles best{0, 0, 0};
+  for (int c = 1; c <= most_c && (c == 1 || (c - 1) * 16 / parts < rows); ++c)  // (a further tile of columns only for rows that the ones before do not hold)
     for (int r = c == 1 ? 1 : 2; r <= 4; ++r) {  // (one tile of outputs with several of columns comes out best for next to nothing)
-      const long rows = c * 16 / XType<XT>::P, p = (a.M + rows - 1) / rows, rounds = ((nt + r - 1) / r * p + 255) / 256;
-      const float more = c == 1 && r == 1 && rounds == 2 && few ? .25f : c == 1 ? more1[r - 1] : a.K < 8192 ? .4f : .6f;
+      const long held = c * 16 / parts, p = (rows + held - 1) / held, rounds = ((nt + r - 1) / r * p + 255) / 256;
+      const float more = c == 1 && r == 1 && rounds == 2 && few ? .25f : c == 1 ? more1[r - 1] : k < 8192 ? .4f : .6f;
       const float t = first[c - 1][r - 1] * (1.f + more * (float)(rounds - 1));
-      if (best < 0 || t < least) least = t, best = 4 * c + r - 5, passes = (int)p;
+      if (best.c == 0 || t < least) least = t, best = {r, c, (int)p};
     }
-  switch (best) {
-    case 0: return go<XT, GJ, 1, 1>(a, passes, st);
-    case 1: return go<XT, GJ, 2, 1>(a, passes, st);
-    case 2: return go<XT, GJ, 3, 1>(a, passes, st);
-    case 3: return go<XT, GJ, 4, 1>(a, passes, st);
-    case 5: return go<XT, GJ, 2, 2>(a, passes, st);
-    case 6: return go<XT, GJ, 3, 2>(a, passes, st);
-    case 7: return go<XT, GJ, 4, 2>(a, passes, st);
+  return best;
+}
+template <int XT, int GJ> void with_tiles(const LinearW4Args& a, hipStream_t st) {
+  const Tiles t = pick_tiles(a.M, a.N, a.K, XT);
+  switch (4 * t.c + t.r - 5) {
+    case 0: return go<XT, GJ, 1, 1>(a, t.passes, st);
+    case 1: return go<XT, GJ, 2, 1>(a, t.passes, st);
+    case 2: return go<XT, GJ, 3, 1>(a, t.passes, st);
+    case 3: return go<XT, GJ, 4, 1>(a, t.passes, st);
+    case 5: return go<XT, GJ, 2, 2>(a, t.passes, st);
+    case 6: return go<XT, GJ, 3, 2>(a, t.passes, st);
+    case 7: return go<XT, GJ, 4, 2>(a, t.passes, st);
   }
-  if constexpr (MOST_C == 3) {
-    switch (best) {
-      case 9: return go<XT, GJ, 2, 3>(a, passes, st);
-      case 10: return go<XT, GJ, 3, 3>(a, passes, st);
-      case 11: return go<XT, GJ, 4, 3>(a, passes, st);
+  if constexpr (XT == X_F32) {
+    switch (4 * t.c + t.r - 5) {
+      case 9: return go<XT, GJ, 2, 3>(a, t.passes, st);
+      case 10: return go<XT, GJ, 3, 3>(a, t.passes, st);
+      case 11: return go<XT, GJ, 4, 3>(a, t.passes, st);
     }
   }
 }
@@ -356,4 +362,11 @@ DTF_API int dtf_linear_w4(const LinearW4Args* p, hipStream_t st) {
   else with_group<X_E4M3>(*p, st);
   DTF_CHECK_LAUNCH();
   return 0;
+}
+
+// The tiles that a wave takes for these sizes: 16 * (tiles of 16 columns) + tiles of outputs
+DTF_API int dtf_linear_w4_tiles(long rows, int outputs, int k, int xtype) {
+  if (rows <= 0 || outputs <= 0 || k <= 0 || xtype < 0 || xtype > 2) return ERR;
+  const Tiles t = pick_tiles(rows, outputs, k, xtype);
+  return 16 * t.c + t.r;
 }

@@ -72,3 +72,23 @@ def test_the_native_side_refuses_bad_blocks():
     fn = native.hip().dtf_linear_w4
     fn.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
     assert fn(None, None) == -22 and fn(ctypes.create_string_buffer(256), None) == -22  # nothing, and an argument block of zeros
+
+
+def test_no_tile_of_columns_that_holds_no_row_is_chosen():
+    """16 columns hold 16 rows, of float32 (three columns a row) 5; a further tile of them only for rows that the ones before do not hold.
+    262144 outputs and their neighbours took a second one for a single row."""
+    from distributed_tensorflow_amd import native
+    fn = native.hip().dtf_linear_w4_tiles
+    fn.argtypes = [ctypes.c_long, ctypes.c_int, ctypes.c_int, ctypes.c_int]
+    assert fn(0, 1, 1, 0) == -22 and fn(1, 1, 1, 3) == -22 and fn(1, 0, 1, 0) == -22 and fn(1, 1, 0, 0) == -22
+    widths = {1, 16, 17, 209000, 262144, 524288, (1 << 31) - 17} | {int(16 * 1.11 ** i) + i % 3 for i in range(150)}
+    several = 0
+    for xtype, parts in ((0, 3), (1, 1), (2, 1)):
+        for rows in list(range(1, 36)) + [64, 1000, 327675]:
+            for k in (1, 4096, 8192, 16384):
+                for n in widths:
+                    c, r = divmod(fn(rows, n, k, xtype), 16)
+                    assert 1 <= c <= (3 if xtype == 0 else 2) and (1 if c == 1 else 2) <= r <= 4
+                    assert c == 1 or rows > (c - 1) * 16 // parts, (rows, n, k, xtype, c, r)
+                    several += c > 1
+    assert several > 1000
