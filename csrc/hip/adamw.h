@@ -6,7 +6,7 @@
 struct AdamWLaunch {
   const int64_t* shape;   // [ntensors][2]: elements, place in the arenas
   const void* chunks;     // [nchunks] {tensor, chunk of 2048 elements in it}
-  void* live;             // [ntensors] written by the first kernel for the second
+  void* live;             // [ntensors] written by the first kernel for the second: no two steps in flight may share it
   int* step;              // [ntensors]
   void* m;                // arenas: float, or e4m3 ...
   void* v;                // ... (r = sqrt(v) in 8 bits)

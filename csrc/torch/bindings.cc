@@ -296,7 +296,6 @@ struct AdamWGroup {
     };
     a.shape = reinterpret_cast<const int64_t*>(get("shape"));
     a.chunks = reinterpret_cast<const void*>(get("chunks"));
-    a.live = reinterpret_cast<void*>(get("live"));
     a.step = reinterpret_cast<int*>(get("step"));
     a.m = reinterpret_cast<void*>(get("m"));
     a.v = reinterpret_cast<void*>(get(bits == 8 ? "r" : "v"));
@@ -355,6 +354,9 @@ struct AdamWGroup {
     a.decay = (float)(1.0 - lr * weight_decay);
     a.grad_scale = (float)grad_scale;
     const c10::DeviceGuard guard(params[0].device());
+    // (a step's own, like its graph's: steps over different parameters of a group may run at once, on two streams or from two captured graphs)
+    const Tensor live = at::empty({(int64_t)params.size() * dtf_sizeof_adamw_live()}, params[0].options().dtype(at::kByte));
+    a.live = live.mutable_data_ptr();
     const int rc = dtf_adamw(&a, pp.data(), gg.data(), kind.data(), stream_of(params[0]));
     for (size_t i = 0; i < grads.size(); ++i)
       if (grads[i].defined() && !params[i].is_inference()) params[i].unsafeGetTensorImpl()->bump_version();  // (a backward pass that saved the old values is refused)

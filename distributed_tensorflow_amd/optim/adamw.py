@@ -5,7 +5,9 @@
 
 On a GPU a step is two kernels whatever the number of tensors (``csrc/hip/adamw.hip``): the parameters and gradients stay where the
 program has them, contiguous fp32 or bf16 tensors in any mix, and the moments live in arenas in which every tensor starts at a
-multiple of 256 elements.  The step counters are on the device, so a captured step advances when it is replayed.  bf16 parameters
+multiple of 256 elements.  The step counters are on the device, so a captured step advances when it is replayed (with the learning rate and
+the other settings that it was captured with).  Steps over different parameters of one optimizer share nothing that is written, and may
+run at once: on two streams, or as two captured graphs.  bf16 parameters
 are updated in fp32 and rounded to nearest: an update below half a bf16 step of its parameter is lost, so keep fp32 parameters
 where that matters.
 
@@ -16,7 +18,6 @@ operations.
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
 from typing import Dict, Iterable, Optional, Sequence
 
@@ -27,9 +28,6 @@ from .. import native
 BLOCK = 256    # elements that share a scale; tensors start at multiples of it (BLOCK, CHUNK: csrc/hip/adamw.hip)
 CHUNK = 2048   # elements of a workgroup
 E4M3 = torch.float8_e4m3fn
-
-
-native.register_hip_sig("dtf_sizeof_adamw_live", C.c_int, [])
 
 
 def _i32(x: int) -> int:
@@ -63,8 +61,7 @@ class _Group:
             first = torch.cumsum(counts, 0) - counts
             self.chunks = torch.stack((owner, torch.arange(owner.numel()) - first[owner]), 1).to(torch.int32).to(dev)
             self.shape = torch.tensor(list(zip(self.sizes, self.at)), dtype=torch.int64).to(dev)
-            self.live = torch.empty(len(params) * native.hip().dtf_sizeof_adamw_live(), dtype=torch.uint8, device=dev)
-            places = {"shape": self.shape, "chunks": self.chunks, "live": self.live, "step": self.step, **self.arenas}
+            places = {"shape": self.shape, "chunks": self.chunks, "step": self.step, **self.arenas}
             self.native = native.ext().AdamWGroup(self.params, {k: t.data_ptr() for k, t in places.items()}, self.chunks.shape[0], bits, self.seed)
 
     def views(self, i: int) -> Dict[str, torch.Tensor]:

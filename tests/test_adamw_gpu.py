@@ -199,3 +199,40 @@ def test_refusals_on_the_gpu():
     with pytest.raises(ValueError):
         opt.step(grads=[torch.ones(9, device="cuda")])
     assert opt.arenas()["step"].tolist() == [0] and not p.detach().any()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_two_captured_steps_over_different_parameters_replay_at_once(bits):
+    """What the first kernel of a step leaves for the second is the step's own: another step's begin, which has no gradient for these
+    parameters, must not reach it."""
+    sizes = [40000, 3, 70001, 900]
+    (gpu, opt), (cpu, ref) = _pair(sizes, [F, B], bits)
+    grads = [torch.zeros(n, device="cuda", dtype=p.dtype) for n, p in zip(sizes, gpu)]
+    halves = [[g if i % 2 == half else None for i, g in enumerate(grads)] for half in (0, 1)]
+    graphs = []
+    for half in halves:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            opt.step(grads=half)
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    gen = torch.Generator().manual_seed(9)
+    for t in range(8):
+        new = [torch.randn(n, generator=gen).to(g.dtype) for n, g in zip(sizes, grads)]
+        for g, x in zip(grads, new):
+            g.copy_(x)
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for half in (0, 1):  # and eager steps, each on its stream
+            with torch.cuda.stream(streams[half]):
+                opt.step(grads=halves[half])
+        torch.cuda.synchronize()
+        ref.step(grads=new)
+        ref.step(grads=new)
+        for p, q in zip(gpu, cpu):
+            assert _same(p, q), t
+        for k, x in opt.arenas().items():
+            assert _same(x, ref.arenas()[k]), (t, k)
