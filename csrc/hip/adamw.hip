@@ -245,9 +245,15 @@ __global__ __launch_bounds__(256) void adamw_apply_kernel(const AdamWLaunch a) {
   }
 }
 
-template <typename P, typename G> static void adamw_apply(const AdamWLaunch& a, hipStream_t st) {
-  if (a.bits == 8) hipLaunchKernelGGL((adamw_apply_kernel<P, G, true>), dim3(a.nchunks), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((adamw_apply_kernel<P, G, false>), dim3(a.nchunks), dim3(256), 0, st, a);
+template <typename P, typename G> static void adamw_apply(const AdamWLaunch& all, hipStream_t st) {
+  constexpr int MOST = 1 << 23;  // chunks of a launch: its threads have to be fewer than 2^32 (more are cut off without an error)
+  for (long first = 0; first < all.nchunks; first += MOST) {
+    AdamWLaunch a = all;
+    a.chunks = static_cast<const int2*>(all.chunks) + first;
+    a.nchunks = (int)(all.nchunks - first < MOST ? all.nchunks - first : MOST);
+    if (a.bits == 8) hipLaunchKernelGGL((adamw_apply_kernel<P, G, true>), dim3(a.nchunks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((adamw_apply_kernel<P, G, false>), dim3(a.nchunks), dim3(256), 0, st, a);
+  }
 }
 
 DTF_API int dtf_sizeof_adamw_live() { return (int)sizeof(AdamWLive); }

@@ -236,3 +236,26 @@ def test_two_captured_steps_over_different_parameters_replay_at_once(bits):
             assert _same(p, q), t
         for k, x in opt.arenas().items():
             assert _same(x, ref.arenas()[k]), (t, k)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_more_chunks_than_a_launch_takes(bits):
+    """2^24 chunks of 2048 elements are 2^32 threads.  The table here has that many entries for a tensor of two chunks: the others lie
+    behind its end and are left at once."""
+    from distributed_tensorflow_amd import native
+    n, entries = 2048 + 300, (1 << 24) + 5
+    (gpu, opt), (cpu, ref) = _pair([n], [F], bits)
+    group = opt._groups[0]
+    chunks = torch.zeros(entries, 2, dtype=torch.int32, device="cuda")
+    chunks[:, 1] = 2  # (starts at element 4096)
+    chunks[0, 1], chunks[-1, 1] = 1, 0
+    places = {"shape": group.shape, "chunks": chunks, "step": group.step, **group.arenas}
+    group.native = native.ext().AdamWGroup(group.params, {k: t.data_ptr() for k, t in places.items()}, entries, bits, group.seed)
+    gen = torch.Generator().manual_seed(3)
+    for _ in range(2):
+        g = torch.randn(n, generator=gen)
+        opt.step(grads=[g.cuda()])
+        ref.step(grads=[g])
+        assert _same(gpu[0], cpu[0])
+        for k, x in opt.arenas().items():
+            assert _same(x, ref.arenas()[k]), k
