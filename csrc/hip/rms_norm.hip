@@ -312,9 +312,9 @@ template <typename T> __device__ __forceinline__ float h_at(const RmsNormArgs& a
   if (a.res) v += load_piece<T, 1>(static_cast<const T*>(a.res) + row * a.ld_res + c).get(0);
   return v;
 }
-template <typename T> __global__ __launch_bounds__(1024) void rms_norm_bwd_long_kernel(const RmsNormArgs a) {
+template <typename T> __global__ __launch_bounds__(1024) void rms_norm_bwd_long_kernel(const RmsNormArgs a, long first) {
   __shared__ float slots[16];
-  const long row = blockIdx.x;
+  const long row = first + blockIdx.x;
   const T* dy = static_cast<const T*>(a.dy) + row * a.ld_dy;
   const T* dh = static_cast<const T*>(a.dh) + row * a.ld_dh;
   const float rstd = a.rstd[row];
@@ -377,6 +377,7 @@ template <typename F> bool with_type(const RmsNormArgs& a, F f) {
   if (a.bf16) return with_shape<8>(a.dim, few, [&](auto s) { f(uint16_t{}, s); });
   return with_shape<4>(a.dim, few, [&](auto s) { f(float{}, s); });
 }
+constexpr long MOST = 1L << 21;  // rows of a launch: its threads have to be fewer than 2^32 (more are cut off without an error)
 bool bad(const RmsNormArgs* a) {
   return !a || !a->x || !a->w || !a->y || a->rows <= 0 || a->dim <= 0 || a->rows > 0x7fffffffL || a->ld_x < 0 || a->ld_res < 0 || a->ld_dy < 0 || a->ld_dh < 0;
 }
@@ -414,7 +415,6 @@ static void fwd_rows(const RmsNormArgs& a, hipStream_t st) {
 
 DTF_API int dtf_rms_norm_fwd(const RmsNormArgs* p, hipStream_t st) {
   if (bad(p) || (p->res && !p->h)) return ERR;
-  constexpr long MOST = 1L << 21;  // rows of a launch: its threads have to be fewer than 2^32
   const long size = p->bf16 ? 2 : 4;
   const auto skip = [](auto* q, long bytes) { return q ? (decltype(q))((uintptr_t)q + bytes) : q; };
   for (long r = 0; r < p->rows; r += MOST) {
@@ -468,7 +468,7 @@ DTF_API int dtf_rms_norm_bwd(const RmsNormArgs* p, hipStream_t st) {
   if (!done) {
     auto go = [&](auto type) {
       using T = decltype(type);
-      hipLaunchKernelGGL((rms_norm_bwd_long_kernel<T>), dim3((unsigned)a.rows), dim3(1024), 0, st, a);
+      for (long r = 0; r < a.rows; r += MOST) hipLaunchKernelGGL((rms_norm_bwd_long_kernel<T>), dim3((unsigned)(a.rows - r < MOST ? a.rows - r : MOST)), dim3(1024), 0, st, a, r);
       if (a.part) hipLaunchKernelGGL((rms_norm_dw_long_kernel<T>), dim3(dtf_cdiv(a.dim, 256), a.blocks), dim3(256), 0, st, a);
     };
     if (a.bf16) go(uint16_t{}); else go(float{});

@@ -320,3 +320,21 @@ def test_the_forms_without_a_backward_pass_refuse_one():
     assert h is z and q.requires_grad  # (without a residual h is x, whose gradient is its own)
     layer = autograd.RMSNorm(200).cuda()
     assert hip_ops.rms_norm_e4m3(x, layer.weight)[0].requires_grad  # (its weight has no gradient here either)
+
+
+def test_backward_of_more_long_rows_than_a_launch_takes():
+    """2^22 workgroups of 1024 threads are 2^32 threads (x and dy are one row for all, dx is 137 GB)."""
+    from distributed_tensorflow_amd.ops import hip_ops
+    rows, dim = (1 << 22) + 3, 8196
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 150 << 30:
+        pytest.skip("needs 150 GB of free memory")
+    gen, one, _, w = _inputs(1, dim, F, False)
+    dy = _rand(gen, 1, dim)
+    rstd = 0.5 + torch.rand(rows, generator=gen, device="cuda")
+    dx, _ = hip_ops.rms_norm_backward(dy.expand(rows, dim), one.expand(rows, dim), rstd, w, need_dw=False)
+    for at in list(range(0, rows, 262139)) + [rows - 5]:
+        r = rstd[at:at + 3]
+        check_backward(dx[at:at + 3], None, dy.expand(3, dim), one.expand(3, dim), r, w, None, None)
+    del dx
+    torch.cuda.empty_cache()
