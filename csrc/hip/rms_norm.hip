@@ -11,6 +11,7 @@
 // those in a fixed order (no atomics: the same result on every run).
 #include "common.h"
 #include "rms_norm.h"
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -340,9 +341,9 @@ template <typename T> __global__ __launch_bounds__(256) void rms_norm_dw_long_ke
 }
 
 // dw: 64 columns a workgroup, 16 waves that take every sixteenth row of partial sums; then the waves' sums in order
-__global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* __restrict__ part, float* __restrict__ dw, int blocks, int dim) {
+__global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* __restrict__ part, float* __restrict__ dw, int blocks, int dim, int first) {
   __shared__ float sums[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane, cc = min(c, dim - 1);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = first + blockIdx.x * 64 + lane, cc = min(c, dim - 1);
   float s = 0.f;
 #pragma unroll 8
   for (int b = wave; b < blocks; b += 16) s += part[(long)b * dim + cc];
@@ -377,7 +378,7 @@ template <typename F> bool with_type(const RmsNormArgs& a, F f) {
   if (a.bf16) return with_shape<8>(a.dim, few, [&](auto s) { f(uint16_t{}, s); });
   return with_shape<4>(a.dim, few, [&](auto s) { f(float{}, s); });
 }
-constexpr long MOST = 1L << 21;  // rows of a launch: its threads have to be fewer than 2^32 (more are cut off without an error)
+constexpr long MOST = 1L << 21;  // workgroups of a launch: its threads have to be fewer than 2^32 (more are cut off without an error)
 bool bad(const RmsNormArgs* a) {
   return !a || !a->x || !a->w || !a->y || a->rows <= 0 || a->dim <= 0 || a->rows > 0x7fffffffL || a->ld_x < 0 || a->ld_res < 0 || a->ld_dy < 0 || a->ld_dh < 0;
 }
@@ -474,7 +475,9 @@ DTF_API int dtf_rms_norm_bwd(const RmsNormArgs* p, hipStream_t st) {
     if (a.bf16) go(uint16_t{}); else go(float{});
   }
   DTF_CHECK_LAUNCH();
-  if (a.dw && a.blocks) hipLaunchKernelGGL(rms_norm_dw_kernel, dim3(dtf_cdiv(a.dim, 64)), dim3(1024), 0, st, a.part, a.dw, a.blocks, a.dim);
+  if (a.dw && a.blocks)
+    for (long c = 0; c < a.dim; c += 64 * MOST)
+      hipLaunchKernelGGL(rms_norm_dw_kernel, dim3((unsigned)((std::min(a.dim - c, 64 * MOST) + 63) / 64)), dim3(1024), 0, st, a.part, a.dw, a.blocks, a.dim, (int)c);
   DTF_CHECK_LAUNCH();
   return 0;
 }

@@ -338,3 +338,17 @@ def test_backward_of_more_long_rows_than_a_launch_takes():
         check_backward(dx[at:at + 3], None, dy.expand(3, dim), one.expand(3, dim), r, w, None, None)
     del dx
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("rows", [1, 2])
+def test_dw_of_more_columns_than_a_launch_takes(rows):
+    """2^28 columns, 64 a workgroup of 1024 threads, are 2^32 threads."""
+    from distributed_tensorflow_amd.ops import hip_ops
+    dim = (1 << 28) + 70
+    gen = torch.Generator("cuda").manual_seed(0)
+    x, dy, w = _rand(gen, rows, dim, dtype=B), _rand(gen, rows, dim, dtype=B), torch.ones(dim, device="cuda")
+    rstd = torch.full((rows,), 0.75, device="cuda")
+    dw = hip_ops.rms_norm_backward(dy, x, rstd, w)[1]
+    for at in list(range(0, dim, (1 << 22) - 3)) + [dim - 80]:  # a product and its sum of two rows, one rounding each
+        h, d = x[:, at:at + 80].double() * 0.75, dy[:, at:at + 80].double()
+        assert bool(((dw[at:at + 80].double() - (h * d).sum(0)).abs() <= (h * d).abs().sum(0) * 4 * 2.0 ** -24).all()), at
