@@ -18,3 +18,4 @@ struct LinearW4Args {
 
 extern "C" int dtf_linear_w4(const LinearW4Args* a, hipStream_t st);
 extern "C" int dtf_linear_w4_tiles(long rows, int outputs, int k, int xtype);
+extern "C" int dtf_linear_w4_waves(long rows, int outputs, int k, int xtype);

@@ -15,6 +15,7 @@
 // results in LDS, in the waves' order.
 #include "common.h"
 #include "linear_w4.h"
+#include <algorithm>
 
 namespace {
 constexpr int ERR = -22;
@@ -278,14 +279,18 @@ template <int XT, int GJ, int R, int C, int PIECES> __global__ __launch_bounds__
 }
 
 namespace {
+// Eight waves split k (4: 11.1 instead of 7.5 us for one row of 16384 by 2048 outputs), twelve where k is long and the CUs have one workgroup each
+// at most (6.5; 15: 6.6; with 4096 k 3.5 instead of 3.4).  Four where each has more to do, and its registers and LDS are more (7: 17.7 instead
+// of 15.6 us for 32 rows bf16, 4096 x 16384).  Fewer where a launch would have 2^32 threads (they are cut off without an error).
+int pick_waves(long groups, long passes, int r, int c, int kt) {
+  const int most = c > 1 ? 4 : r == 1 && kt >= 64 && groups * passes <= 256 ? 12 : 8;
+  return (int)std::min<long>(std::min(kt, most), 0xffffffffL / (64 * groups));
+}
 template <int XT, int GJ, int R, int C> void go(const LinearW4Args& a, int passes, hipStream_t st) {
   constexpr int ROW = 128 * sizeof(typename XType<XT>::T), MC = C * 16 / XType<XT>::P, MOST = (MC * ROW + 1023) / 1024;  // bytes of a tile's row; KB of a tile
-  // eight waves split k (4: 11.1 instead of 7.5 us for one row of 16384 by 2048 outputs), twelve where k is long and the CUs have one workgroup each
-  // at most (6.5; 15: 6.6; with 4096 k 3.5 instead of 3.4).  Four where each has more to do, and its registers and LDS are more (7: 17.7 instead
-  // of 15.6 us for 32 rows bf16, 4096 x 16384)
   const int nt = (a.N + 15) / 16, kt = (a.K + 127) / 128;
   const dim3 grid((nt + R - 1) / R, passes);
-  const int most = C > 1 ? 4 : R == 1 && kt >= 64 && (long)nt * passes <= 256 ? 12 : 8, waves = kt < most ? kt : most;
+  const int waves = pick_waves(grid.x, passes, R, C, kt);
   static_assert(32 * PITCH >= R * 1024, "a wave's sums take the place of its tiles of x");
   const int lds = 32 * PITCH * C * waves;
   if constexpr (C == 1) {
@@ -369,4 +374,10 @@ DTF_API int dtf_linear_w4_tiles(long rows, int outputs, int k, int xtype) {
   if (rows <= 0 || outputs <= 0 || k <= 0 || xtype < 0 || xtype > 2) return ERR;
   const Tiles t = pick_tiles(rows, outputs, k, xtype);
   return 16 * t.c + t.r;
+}
+// The waves of each of its workgroups
+DTF_API int dtf_linear_w4_waves(long rows, int outputs, int k, int xtype) {
+  if (rows <= 0 || outputs <= 0 || k <= 0 || xtype < 0 || xtype > 2) return ERR;
+  const Tiles t = pick_tiles(rows, outputs, k, xtype);
+  return pick_waves((((long)outputs + 15) / 16 + t.r - 1) / t.r, t.passes, t.r, t.c, (int)(((long)k + 127) / 128));
 }

@@ -92,3 +92,21 @@ def test_no_tile_of_columns_that_holds_no_row_is_chosen():
                     assert c == 1 or rows > (c - 1) * 16 // parts, (rows, n, k, xtype, c, r)
                     several += c > 1
     assert several > 1000
+
+
+def test_a_launch_stays_below_two_to_the_32_threads():
+    """More are cut off without an error: 800 M outputs of 512 k (206 GB of weights) took 2^32 and more."""
+    from distributed_tensorflow_amd import native
+    tiles, waves = native.hip().dtf_linear_w4_tiles, native.hip().dtf_linear_w4_waves
+    for fn in (tiles, waves):
+        fn.argtypes = [ctypes.c_long, ctypes.c_int, ctypes.c_int, ctypes.c_int]
+    assert waves(0, 1, 1, 0) == -22 and waves(1, 1, 1, 3) == -22
+    for xtype in (0, 1, 2):
+        for rows in (1, 2, 5, 6, 16, 17, 33, 327675):
+            for k in (1, 128, 129, 512, 2048, 16384):
+                for n in (1, 2048, 1 << 20, 805306368, 805306369, 900000000, 1 << 30, (1 << 31) - 18):
+                    r = tiles(rows, n, k, xtype) % 16
+                    groups, w = -(-(-(-n // 16)) // r), waves(rows, n, k, xtype)
+                    assert 1 <= w <= min(12, -(-k // 128)) and groups * 64 * w < 1 << 32, (xtype, rows, k, n, r, w)
+    # where the limit is far, as many as the sizes ask for
+    assert waves(1, 2048, 16384, 1) == 12 and waves(1, 8192, 8192, 1) == 8 and waves(16, 16384, 16384, 0) == 4 and waves(3, 100, 300, 1) == 3
