@@ -110,3 +110,20 @@ def test_a_launch_stays_below_two_to_the_32_threads():
                     assert 1 <= w <= min(12, -(-k // 128)) and groups * 64 * w < 1 << 32, (xtype, rows, k, n, r, w)
     # where the limit is far, as many as the sizes ask for
     assert waves(1, 2048, 16384, 1) == 12 and waves(1, 8192, 8192, 1) == 8 and waves(16, 16384, 16384, 0) == 4 and waves(3, 100, 300, 1) == 3
+
+
+def test_a_layers_buffers_keep_their_types_through_casts_of_the_model():
+    """wq, scales and bias are a format: a model's float(), half() or to(bfloat16) turned scales and bias into types that the kernel refuses."""
+    from distributed_tensorflow_amd.ops import autograd
+    layer = autograd.LinearW4.from_linear(autograd.Linear(130, 20), 32)
+    want = {k: t.clone() for k, t in layer.state_dict().items()}
+    model = torch.nn.Sequential(torch.nn.Linear(4, 4), layer)
+    for cast in (lambda m: m.float(), lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.double(), lambda m: m.to(torch.bfloat16), lambda m: m.to("cpu"),
+                 lambda m: m.float()):
+        cast(model)
+        assert list(layer.state_dict()) == list(want)
+        for k, t in layer.state_dict().items():
+            assert t.dtype == want[k].dtype and torch.equal(t.view(torch.uint8), want[k].view(torch.uint8)), k
+    assert model[0].weight.dtype == torch.float32  # the last cast
+    meta = model.to("meta")[1]
+    assert all(t.is_meta and t.dtype == want[k].dtype for k, t in meta.state_dict().items())
