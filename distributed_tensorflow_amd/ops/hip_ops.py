@@ -416,7 +416,8 @@ def linear_w4(x: torch.Tensor, wq: torch.Tensor, scales: torch.Tensor, out_featu
     """``relu?((x * x_scale) @ W + bias)`` with the weights of ``quantize_w4``, for inference: made for a single row and a few dozen.
 
     ``x[..., K]`` fp32 (not rounded), bf16, or e4m3 with ``x_scale`` (fp32, one a row; as ``rms_norm_e4m3`` gives them; optional for
-    the other types); any stride between rows.  ``bias`` fp32 ``[out_features]``; the result fp32 or bf16 ``[..., out_features]``.  Sums are fp32.
+    the other types); any stride between rows.  ``bias`` fp32 ``[out_features]``; the result fp32 or bf16 ``[..., out_features]``.  Sums are fp32, and
+    the products of x and the codes of a group are summed before its scale: where that sum passes 3.4e38 (never while |x| < 4e35) the result is infinite or NaN.
     More rows than 16 (fp32: 5), or 32 (fp32: 16) where the outputs are many enough, read the weights again.  Where an operand requires a
     gradient the result does too, and its backward pass raises: there is none."""
     if out_dtype not in (torch.float32, torch.bfloat16):

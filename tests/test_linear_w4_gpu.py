@@ -254,3 +254,21 @@ def test_operands_that_require_a_gradient_make_the_backward_pass_raise(which):
         hidden = first(x.detach())
         with pytest.raises(RuntimeError, match="no backward pass"):
             (last(hidden).sum() + hidden.sum()).backward()
+
+
+@pytest.mark.parametrize("dtype", [F, B])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_large_values_up_to_where_a_groups_products_overflow(group, dtype):
+    """A group's products are summed in fp32 before its scale: they have to be finite there, as 6 * group * |x| is for the values here.  (The largest
+    values of the type itself, times a code of up to 6, are not.)"""
+    from distributed_tensorflow_amd.ops import hip_ops
+    wq, scales = hip_ops.quantize_w4(0.02 * torch.randn(300, 40, generator=torch.Generator("cuda").manual_seed(0), device="cuda"), group)
+    w = hip_ops.dequantize_w4(wq, scales, 300, 40).double()
+    top = torch.finfo(F).max
+    sign = torch.where(torch.rand(5, 300, generator=torch.Generator("cuda").manual_seed(1), device="cuda") < 0.5, -1.0, 1.0)
+    x = (sign * (top / (8 * group))).to(dtype)
+    assert float(w.abs().amax()) < 0.2  # (300 / 256 of that: the sum over the groups stays finite too)
+    check(hip_ops.linear_w4(x, wq, scales, 40), x, None, w, None, False)
+    z = torch.zeros(3, 300, device="cuda").to(dtype)
+    z[:, 7] = top / 8  # alone in its group
+    check(hip_ops.linear_w4(z, wq, scales, 40), z, None, w, None, False)
