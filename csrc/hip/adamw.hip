@@ -5,13 +5,15 @@
 //
 // A step streams p, g and the moments once: 28 bytes an element (fp32, 32-bit moments) down to 10 (bf16, 8-bit moments).  The
 // parameters and gradients are wherever the program put them; the moments lie in arenas in which every tensor starts at a multiple
-// of 256 elements.  Two kernels a step: `begin` takes the pointers by value (a captured graph keeps them, and nothing is kept by an
+// of 256 elements.  Two kernels a step (`begin` once for every 200 tensors, `apply` once for every pair of parameter and gradient types in use): `begin` takes the pointers by value (a captured graph keeps them, and nothing is kept by an
 // address from one call to the next), advances every tensor's step counter and works out its bias corrections; `apply` runs over a
 // fixed list of 2048-element chunks of all tensors.
 //
 // Measured: 190 tensors of 24 M fp32 elements, 8-bit moments, 72 us (5.3 TB/s); 64 of 268 M bf16 elements 494-545 us (5.0-5.5 TB/s), where about
 // 65 issue slots an element keep the vector units two thirds busy (at 105, before the conversion and the root were shortened, they were
-// the bound: 678 us); MNIST's eight tensors with 32-bit moments 18.5 us (5.0 TB/s).
+// the bound: 678 us); MNIST's eight tensors with 32-bit moments 18.5 us (5.0 TB/s).  Where a tensor or its gradient does not start at a multiple of 16
+// bytes its elements are moved one by one: the 268 M as 64 allocations of their own, all values random, 490-600 us, one element further on 820-860.
+// A second pair of types is a second launch over all chunks, whose workgroups leave at once where it is not theirs: 38-41 us for 131 000.
 //
 // 8-bit moments: 256 elements share a scale.  m and r = sqrt(v) (the root halves the range that the code has to span) are e4m3 times
 // a power of two that brings the block's largest magnitude into [128, 256).  They are rounded stochastically, with 16 bits of a hash
@@ -28,7 +30,7 @@
 namespace {
 constexpr int BLOCK = 256;    // elements that share a scale
 constexpr int CHUNK = 2048;   // elements of a workgroup: 8 a lane, so that 16-bit operands move 16 bytes a lane
-constexpr int NARGS = 200;    // tensors whose pointers fit the arguments of one `begin` launch
+constexpr int NARGS = 200;    // tensors whose pointers one `begin` launch takes (its arguments, 4096 bytes, would hold 232)
 }  // namespace
 
 struct AdamWLive {  // what `begin` leaves for `apply`, one a tensor
@@ -126,8 +128,8 @@ constexpr uint32_t INF_BITS = 0x7f800000u;
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 __device__ __forceinline__ uint32_t finite_magnitude(float x) { return magnitude(x) < INF_BITS ? magnitude(x) : 0u; }
 
-// The nearest float to sqrt(x) for x = 0, infinity, NaN and from 2^-96 on (every mantissa was checked): v_sqrt_f32 is at most one step off,
-// and the signs of x - (s - step) s and x - (s + step) s say which neighbour is right.  sqrtf also scales small arguments: 19 instead of
+// The nearest float to sqrt(x) for x = 0, infinity, NaN and from 2^-96 on, by Tuckerman's rounding test: v_sqrt_f32 is at most one step off,
+// and the signs of x - (s - step) s and x - (s + step) s say which neighbour is right.  (The tests compare moments with the CPU's nearest root, bit for bit.)  sqrtf also scales small arguments: 19 instead of
 // 9 instructions, which count here (see adamw_apply_kernel).
 __device__ __forceinline__ float sqrt_from_2_96(float x) {
   const float s = __builtin_amdgcn_sqrtf(x), lo = __uint_as_float(__float_as_uint(s) - 1u), hi = __uint_as_float(__float_as_uint(s) + 1u);

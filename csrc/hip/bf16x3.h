@@ -17,8 +17,8 @@ __device__ __forceinline__ f32x4 mfma16bf(bf16x8 a, bf16x8 b, f32x4 c) {
 
 struct Bf3Pair { uint32_t p0, p1, p2; };  // (lo, hi) of two values, per plane
 
-// (two values per v_cvt_pk_bf16_f32 and per v_pk_add_f32: 10 VALU operations per pair; converting the values one by one and
-// OR-ing the halves together, as pack_bf2 compiles, takes 15)
+// (two values per v_cvt_pk_bf16_f32: 11 VALU operations per pair, the differences one by one, as the build allows no packed fp32
+// instructions; converting the values one by one and OR-ing the halves together, as pack_bf2 compiles, takes 5 more)
 typedef __bf16 bf16x2_x3 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t bf3_pack2(const f32x2 v) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_x3));

@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void conv1_fwd_kernel(const float* __restrict_
       patch[r][c] = t.x;
       patch[r][c + 1] = t.y;
     }
-  // channel pairs on v_pk_fma_f32 (two fp32 fmas per lane and instruction: this loop is the kernel's VALU time)
+  // channel pairs (this loop is the kernel's VALU time; one v_fma_f32 for each of a pair, as the build allows no packed fp32 instructions)
   f32x2 acc2[4][4];
 #pragma unroll
   for (int s = 0; s < 4; ++s)

@@ -3,7 +3,8 @@
     m = b1*m + (1-b1)*g ;  v = b2*v + (1-b2)*g*g
     p = p*(1 - lr*weight_decay) - lr * (m / (1-b1^t)) / (sqrt(v / (1-b2^t)) + eps)
 
-On a GPU a step is two kernels whatever the number of tensors (``csrc/hip/adamw.hip``): the parameters and gradients stay where the
+On a GPU a step is two kernels (``csrc/hip/adamw.hip``; the first once for every 200 tensors, the second once for every pair of parameter and
+gradient types in use): the parameters and gradients stay where the
 program has them, contiguous fp32 or bf16 tensors in any mix, and the moments live in arenas in which every tensor starts at a
 multiple of 256 elements.  The step counters are on the device, so a captured step advances when it is replayed (with the learning rate and
 the other settings that it was captured with).  Steps over different parameters of one optimizer share nothing that is written, and may

@@ -1,5 +1,5 @@
 """Diagnostic: phase timestamps of every workgroup of the fp32 conv2 data-gradient and filter-gradient kernels.
-Build (CPU box): hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared -DDTF_CONV_STAMPS -I csrc/hip csrc/hip/f32_conv2.hip -o scripts/dbg/libf32conv_stamps.so"""
+Build (CPU box): hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC -shared -DDTF_CONV_STAMPS -I csrc/hip csrc/hip/f32_conv2.hip -o scripts/dbg/libf32conv_stamps.so"""
 import ctypes as C, os
 import numpy as np, torch
 here = os.path.dirname(os.path.abspath(__file__))

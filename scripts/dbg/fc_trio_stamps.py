@@ -1,5 +1,5 @@
 """Diagnostic: phase timestamps of every workgroup of the fp32 fc backward launch (fc1 data gradient split-K + fc1 dW + fc2 dW).
-Build (CPU box): hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared -DDTF_GEMM32_STAMPS -I csrc/hip csrc/hip/f32_fc.hip -o scripts/dbg/libf32fc_stamps.so"""
+Build (CPU box): hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC -shared -DDTF_GEMM32_STAMPS -I csrc/hip csrc/hip/f32_fc.hip -o scripts/dbg/libf32fc_stamps.so"""
 import ctypes as C, os
 import numpy as np, torch
 here = os.path.dirname(os.path.abspath(__file__))

@@ -15,7 +15,7 @@ tmp = tempfile.mkdtemp()
 procs = []
 for src in sorted(glob.glob(os.path.join(ROOT, "csrc", "hip", "*.hip"))):
     out = os.path.join(tmp, os.path.basename(src)[:-4] + ".s")
-    procs.append((src, out, subprocess.Popen(["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "--cuda-device-only", "-S", src,
+    procs.append((src, out, subprocess.Popen(["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "--cuda-device-only", "-S", src,
                                               "-o", out, "-I", os.path.join(ROOT, "csrc", "hip")], stderr=subprocess.DEVNULL)))
 load = re.compile(r"\b(global_load|buffer_load|flat_load|scratch_load)")
 found = 0

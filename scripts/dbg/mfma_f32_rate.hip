@@ -1,6 +1,6 @@
 // Micro-benchmark: sustained issue rate of v_mfma_f32_16x16x4_f32 with 1 / 2 / 4 waves per SIMD and 10 independent
 // accumulators per wave (the shape of the fp32 conv2 kernels' inner loops, without any memory traffic).
-//   hipcc --offload-arch=gfx950 -O3 scripts/dbg/mfma_f32_rate.hip -o scripts/dbg/mfma_f32_rate && scripts/dbg/mfma_f32_rate
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops scripts/dbg/mfma_f32_rate.hip -o scripts/dbg/mfma_f32_rate && scripts/dbg/mfma_f32_rate
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef float f32x4 __attribute__((ext_vector_type(4)));

@@ -1,5 +1,5 @@
 """Diagnostic: phase timestamps of every workgroup of the bf16x6 conv2 forward (shader clock + 100 MHz real-time clock).
-Build (CPU box): hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared -DDTF_CONV_STAMPS -I csrc/hip csrc/hip/f32x3_conv2.hip -o scripts/dbg/libx3conv_stamps.so"""
+Build (CPU box): hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC -shared -DDTF_CONV_STAMPS -I csrc/hip csrc/hip/f32x3_conv2.hip -o scripts/dbg/libx3conv_stamps.so"""
 import ctypes as C, os
 import numpy as np, torch
 here = os.path.dirname(os.path.abspath(__file__))
