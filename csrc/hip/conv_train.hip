@@ -180,11 +180,15 @@ __global__ __launch_bounds__(256) void bn_finalize_relu_fwd_kernel(const float* 
                                                                    float inv_count, float eps, float momentum) {
   extern __shared__ float sm[];  // scale[C], shift[C]
   for (int c = threadIdx.x; c < C; c += 256) {
+    float slot[2 * DTF_STAT_SLOTS];  // (all loads first: scheduled with the sums, the compiler waits for them one by one)
+#pragma unroll
+    for (int k = 0; k < 2 * DTF_STAT_SLOTS; ++k) slot[k] = stats[k * C + c];
+    __builtin_amdgcn_sched_barrier(0);
     float s = 0.f, ss = 0.f;
 #pragma unroll
     for (int k = 0; k < DTF_STAT_SLOTS; ++k) {
-      s += stats[(2 * k) * C + c];
-      ss += stats[(2 * k + 1) * C + c];
+      s += slot[2 * k];
+      ss += slot[2 * k + 1];
     }
     const float mean = s * inv_count;
     const float var = fmaxf(ss * inv_count - mean * mean, 0.f);

@@ -11,12 +11,13 @@ import glob, os, re, subprocess, sys, tempfile
 
 ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 min_run = int(sys.argv[1]) if len(sys.argv) > 1 else 4
+sys.path.insert(0, ROOT)
+from distributed_tensorflow_amd import build  # noqa: E402  (the library's own compiler line: other flags, other code)
 tmp = tempfile.mkdtemp()
 procs = []
 for src in sorted(glob.glob(os.path.join(ROOT, "csrc", "hip", "*.hip"))):
     out = os.path.join(tmp, os.path.basename(src)[:-4] + ".s")
-    procs.append((src, out, subprocess.Popen(["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "--cuda-device-only", "-S", src,
-                                              "-o", out, "-I", os.path.join(ROOT, "csrc", "hip")], stderr=subprocess.DEVNULL)))
+    procs.append((src, out, subprocess.Popen(build._recipe("hip")[2] + ["--cuda-device-only", "-S", src, "-o", out], stderr=subprocess.DEVNULL)))
 load = re.compile(r"\b(global_load|buffer_load|flat_load|scratch_load)")
 found = 0
 for src, out, p in procs:
