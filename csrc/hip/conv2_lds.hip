@@ -50,15 +50,15 @@ __global__ __launch_bounds__(256) void conv2_fwd_lds_kernel(const uint16_t* __re
 
   // ---- one burst of loads: image chunks (6 per thread, halo -> zero) + filter slice (25 float4 per thread)
   uint4 iv[6];
+  bool ok[6];
 #pragma unroll
   for (int i = 0; i < 6; ++i) {
     const int c = tid + 256 * i;  // 1296 payload chunks (324 pixels x 4)
     const int pix = c >> 2, q = c & 3;
     const int hy = pix / 18, hx = pix - hy * 18;
     const int y = hy - 2, xx = hx - 2;
-    const bool ok = c < 1296 && (unsigned)y < 14u && (unsigned)xx < 14u;
-    iv[i] = *reinterpret_cast<const uint4*>(x + (ok ? (((long)b * 14 + y) * 14 + xx) * 32 + q * 8 : 0L));
-    if (!ok) iv[i] = make_uint4(0, 0, 0, 0);
+    ok[i] = c < 1296 && (unsigned)y < 14u && (unsigned)xx < 14u;
+    iv[i] = *reinterpret_cast<const uint4*>(x + (ok[i] ? (((long)b * 14 + y) * 14 + xx) * 32 + q * 8 : 0L));
   }
   u32x4 wv[13];  // this half's packed slice: 51 200 B = 3200 chunks of 16 B, already in LDS order
   const u32x4* wsrc = reinterpret_cast<const u32x4*>(Wf + blockIdx.y * W_BYTES);
@@ -67,9 +67,11 @@ __global__ __launch_bounds__(256) void conv2_fwd_lds_kernel(const uint16_t* __re
     const int c = tid + 256 * j;
     wv[j] = wsrc[c < 3200 ? c : 0];
   }
+  __builtin_amdgcn_sched_barrier(0);  // (all loads first: with the zeros chosen at each, the compiler puts it under a branch and waits for it there)
 #pragma unroll
   for (int i = 0; i < 6; ++i) {
     const int c = tid + 256 * i;
+    if (!ok[i]) iv[i] = make_uint4(0, 0, 0, 0);
     if (c < 1296) *reinterpret_cast<uint4*>(img + (c >> 2) * PIX + (c & 3) * 16) = iv[i];
   }
 #pragma unroll

@@ -58,3 +58,23 @@ def test_bf16x6_kernels_run_on_the_bf16_matrix_cores_without_scratch():
     assert "v_mfma_f32_16x16x32_bf16" in fwd[0] and "ds_read_b64_tr_b16" in fwd[0] and "scratch_" not in fwd[0]
     exact = [b for n, b in fc.items() if "fc_fwd32_kernelILb0ELb0" in n]
     assert len(exact) == 1 and "v_mfma_f32_16x16x4_f32" in exact[0] and "v_mfma_f32_16x16x32_bf16" not in exact[0]
+
+
+@pytest.mark.skipif(shutil.which("hipcc") is None, reason="needs hipcc")
+def test_the_bf16_conv2_forward_issues_its_loads_in_one_burst(tmp_path):
+    """Five pieces of the image (the sixth is halo alone, zeros) and thirteen of the filter: all on their way before the first wait, compiled as
+    the library is built."""
+    sys.path.insert(0, REPO)
+    from distributed_tensorflow_amd import build
+    out = str(tmp_path / "conv2_lds.s")
+    subprocess.run(build._recipe("hip")[2] + ["--cuda-device-only", "-S", os.path.join(REPO, "csrc", "hip", "conv2_lds.hip"), "-o", out], check=True,
+                   stderr=subprocess.DEVNULL, timeout=300)
+    with open(out) as f:
+        text = f.read()
+    body = text[text.index("\n_Z20conv2_fwd_lds_kernel"):]
+    loads = 0
+    for line in body.splitlines():
+        loads += "global_load" in line
+        if "vmcnt(" in line or "s_barrier" in line:
+            break
+    assert loads == 18
