@@ -294,11 +294,10 @@ class LinearW4(nn.Module):
 
     def _apply(self, fn, recurse=True):
         # (a move to another device reaches the buffers, a cast of the model does not: their types are the kernel's format)
-        for name, t in self._buffers.items():
-            if t is not None:
-                out = fn(t)
-                self._buffers[name] = out if out.dtype == t.dtype else t.to(out.device)
-        return self
+        def move(t):
+            out = fn(t)
+            return out if out.dtype == t.dtype else t.to(out.device)
+        return super()._apply(move, recurse)
 
     def forward(self, x, x_scale=None):
         return hip_ops.linear_w4(x, self.wq, self.scales, self.out_features, self.bias, self.relu, x_scale)
