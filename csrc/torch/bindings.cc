@@ -34,6 +34,11 @@ void check(int rc, const char* what) {
 template <typename... Operands> std::shared_ptr<torch::autograd::Node> refusal(const char* message, const Operands&... operands) {
   return std::make_shared<torch::autograd::Error>(message, torch::autograd::collect_next_edges(operands...));
 }
+// Forward mode: what has no rule for tangents refuses them
+template <typename... Operands> void no_tangents(const char* what, const Operands&... operands) {
+  const bool any = (torch::autograd::isFwGradDefined(operands) || ...);
+  TORCH_CHECK_NOT_IMPLEMENTED(!any, what, " has no forward-mode derivative");
+}
 template <typename F> auto without_grad(F f) {
   const at::NoGradGuard no_grad;
   return f();
@@ -116,6 +121,7 @@ void refuse_backward(const std::tuple<Tensor, Tensor, Tensor>& out, const OptTen
   if (residual) torch::autograd::set_history(std::get<2>(out), fn);
 }
 std::tuple<Tensor, Tensor, Tensor> rms_norm_forward(const Tensor& x, const Tensor& w, const OptTensor& residual, double eps) {
+  no_tangents("rms_norm_forward", OptTensor(x), residual);
   const auto out = without_grad([&] { return norm_forward(x, w, residual, eps, false); });
   // (not the weight: a layer's parameter is passed as it is by those who call rms_norm_backward themselves)
   refuse_backward(out, residual, "rms_norm_forward has no backward pass of its own: autograd.rms_norm has", x, residual);
@@ -123,6 +129,7 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_forward(const Tensor& x, const Tenso
   return {y, h, rstd};
 }
 std::tuple<Tensor, Tensor, Tensor> rms_norm_e4m3(const Tensor& x, const Tensor& w, const OptTensor& residual, double eps) {
+  no_tangents("rms_norm_e4m3", OptTensor(x), OptTensor(w), residual);
   const auto out = without_grad([&] { return norm_forward(x, w, residual, eps, true); });
   refuse_backward(out, residual, "rms_norm_e4m3 is for inference: it has no backward pass", x, w, residual);
   return out;
@@ -268,6 +275,7 @@ Tensor w4_product(const Tensor& x, const Tensor& wq, const Tensor& scales, int64
 }
 Tensor linear_w4(const Tensor& x, const Tensor& wq, const Tensor& scales, int64_t N, const OptTensor& bias, bool relu, const OptTensor& x_scale,
                  bool out_bf16) {
+  no_tangents("linear_w4", OptTensor(x), bias, x_scale);
   const Tensor y = w4_product(x, wq, scales, N, bias, relu, x_scale, out_bf16);
   if (torch::autograd::compute_requires_grad(x, scales, bias, x_scale))
     torch::autograd::set_history(y, refusal("linear_w4 is for inference: it has no backward pass", x, scales, bias, x_scale));

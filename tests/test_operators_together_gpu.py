@@ -126,3 +126,19 @@ def test_a_captured_training_step_replays_like_eager():
         assert torch.equal(w1, w2)
         for k, t in o1.arenas().items():
             assert torch.equal(t.view(torch.uint8), o2.arenas()[k].view(torch.uint8))
+
+
+def test_forward_mode_derivatives_are_refused():
+    """Tangents were dropped without a word where there is no rule for them; autograd.rms_norm's node refuses them itself."""
+    import torch.autograd.forward_ad as fwd
+    from distributed_tensorflow_amd.ops import autograd as ag, hip_ops
+    x, w, t = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda"), torch.randn(4, 64, device="cuda")
+    wq, scales = hip_ops.quantize_w4(torch.randn(64, 32, device="cuda"))
+    with fwd.dual_level():
+        d = fwd.make_dual(x, t)
+        for f in (lambda: ag.rms_norm(d, w), lambda: hip_ops.rms_norm_forward(d, w), lambda: hip_ops.rms_norm_forward(x, w, d),
+                  lambda: hip_ops.rms_norm_e4m3(d, w), lambda: hip_ops.rms_norm_e4m3(x, fwd.make_dual(w, w)),
+                  lambda: hip_ops.linear_w4(d, wq, scales, 32), lambda: hip_ops.linear_w4(x, wq, scales, 32, bias=fwd.make_dual(w[:32], w[:32]))):
+            with pytest.raises(RuntimeError, match="forward-mode|jvp"):
+                f()
+        assert hip_ops.linear_w4(x, wq, scales, 32).shape == (4, 32)
