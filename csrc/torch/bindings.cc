@@ -48,7 +48,7 @@ bool is_rows(const Tensor& t) {
 }
 // A side operand: fp32, contiguous, of n elements on like's device
 void check_f32(const Tensor& t, const char* name, int64_t n, const Tensor& like) {
-  TORCH_CHECK_VALUE(t.is_cuda() && t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == n && t.device() == like.device(), name,
+  TORCH_CHECK_VALUE(t.is_cuda() && t.scalar_type() == at::kFloat && t.is_contiguous() && !t.is_neg() && t.numel() == n && t.device() == like.device(), name,
                     " must be a contiguous CUDA tensor of ", n, " float32 values on ", like.device(), " (got ", t.scalar_type(), " ", t.sizes(),
                     " on ", t.device(), ")");
 }
@@ -65,13 +65,13 @@ struct Rows {  // rows of the last dimension: any stride between rows, none insi
                       t.scalar_type(), " ", t.sizes(), " on ", t.device(), ") must have the type, shape and device of the other rows");
     if (t.numel() == 0) return;
     keep = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
-    if (keep.size(1) > 1 && keep.stride(1) != 1) keep = keep.contiguous();
+    if (keep.is_neg() || (keep.size(1) > 1 && keep.stride(1) != 1)) keep = keep.resolve_neg().contiguous();  // (the imaginary part of a conjugate: negated lazily)
     p = keep.const_data_ptr();
     ld = keep.stride(0);
   }
 };
 void check_weight(const Tensor& w, const Tensor& x, double eps) {
-  TORCH_CHECK_VALUE(w.is_cuda() && w.scalar_type() == at::kFloat && w.is_contiguous() && w.dim() == 1 && w.device() == x.device() && w.size(0) >= 1 &&
+  TORCH_CHECK_VALUE(w.is_cuda() && w.scalar_type() == at::kFloat && w.is_contiguous() && !w.is_neg() && w.dim() == 1 && w.device() == x.device() && w.size(0) >= 1 &&
                         x.size(-1) == w.size(0),
                     "weight must be contiguous float32 of the rows' length on their device (got ", w.scalar_type(), " ", w.sizes(), " on ",
                     w.device(), " for rows ", x.sizes(), " on ", x.device(), ")");
@@ -254,7 +254,7 @@ Tensor w4_product(const Tensor& x, const Tensor& wq, const Tensor& scales, int64
   const Tensor y = at::empty(shape, x.options().dtype(out_bf16 ? at::kBFloat16 : at::kFloat));
   if (M == 0) return y;
   Tensor rows = x.dim() == 2 ? x : x.reshape({-1, K});
-  if (K > 1 && rows.stride(1) != 1) rows = rows.contiguous();
+  if (rows.is_neg() || (K > 1 && rows.stride(1) != 1)) rows = rows.resolve_neg().contiguous();
   LinearW4Args a{};
   a.x = rows.const_data_ptr();
   a.wq = wq.const_data_ptr();
@@ -327,7 +327,7 @@ struct AdamWGroup {
     bool any = false;
     for (size_t i = 0; i < n; ++i) {
       const Tensor& t = params[i];
-      TORCH_CHECK_VALUE(t.scalar_type() == types[i] && t.numel() == sizes[i] && t.device() == device && t.is_contiguous(),
+      TORCH_CHECK_VALUE(t.scalar_type() == types[i] && t.numel() == sizes[i] && t.device() == device && t.is_contiguous() && !t.is_neg(),
                         "a parameter's type, size, device or layout has changed since it was given to AdamW");
       Tensor d = given ? (*given)[i].value_or(Tensor()) : t.grad();
       if (!d.defined()) continue;
@@ -336,7 +336,7 @@ struct AdamWGroup {
       TORCH_CHECK_VALUE(d.device() == device && d.sizes() == t.sizes(), "a gradient of shape ", d.sizes(), " on ", d.device(),
                         " for a parameter of shape ", t.sizes(), " on ", device);
       if (sizes[i] == 0) continue;
-      found[i] = d.is_contiguous() ? d : d.contiguous();
+      found[i] = d.resolve_neg().contiguous();
       p[i] = reinterpret_cast<uint64_t>(t.data_ptr());
       g[i] = reinterpret_cast<uint64_t>(found[i].const_data_ptr());
       k[i] = (types[i] == at::kBFloat16 ? 1 : 0) | (d.scalar_type() == at::kBFloat16 ? 2 : 0);

@@ -192,7 +192,7 @@ class AdamW(torch.optim.Optimizer):
         if len(set(map(id, grp["params"]))) < len(grp["params"]):
             raise ValueError("a parameter is twice in one group")
         for p in grp["params"]:
-            if p.dtype not in (torch.float32, torch.bfloat16) or p.layout != torch.strided or not p.is_contiguous():
+            if p.dtype not in (torch.float32, torch.bfloat16) or p.layout != torch.strided or not p.is_contiguous() or p.is_neg():
                 raise ValueError("AdamW takes contiguous float32 or bfloat16 parameters (got %s, strides %s)" % (p.dtype, tuple(p.stride())))
             if p.device != grp["params"][0].device or p.device.type not in ("cpu", "cuda"):
                 raise ValueError("a group's parameters share one device, a GPU or the CPU")

@@ -142,3 +142,28 @@ def test_forward_mode_derivatives_are_refused():
             with pytest.raises(RuntimeError, match="forward-mode|jvp"):
                 f()
         assert hip_ops.linear_w4(x, wq, scales, 32).shape == (4, 32)
+
+
+def test_lazily_negated_views():
+    """The imaginary part of a conjugate is a view whose memory holds the other sign; with one element a row it passes for contiguous."""
+    from distributed_tensorflow_amd.ops import hip_ops
+    from distributed_tensorflow_amd.optim.adamw import AdamW
+    z = torch.randn(3, 1, dtype=torch.complex64, device="cuda")
+    x, plain = z.conj().imag, -z.imag.clone()
+    assert x.is_neg() and not plain.is_neg()
+    one = torch.ones(1, device="cuda")
+    y, h, rstd = hip_ops.rms_norm_forward(x, one, x)
+    check_forward(y, h, rstd, plain, one, plain, 1e-6)
+    check_e4m3(*hip_ops.rms_norm_e4m3(x, one)[:2], plain, one, None, 1e-6)
+    check_backward(*hip_ops.rms_norm_backward(x, x, rstd, one, x, x), plain, plain, rstd, one, plain, plain)
+    wq, scales = hip_ops.quantize_w4(torch.ones(1, 20, device="cuda"), 32)
+    assert torch.equal(hip_ops.linear_w4(x, wq, scales, 20), hip_ops.linear_w4(plain, wq, scales, 20))
+    ps = [torch.zeros(1, 1, device="cuda", requires_grad=True) for _ in range(2)]
+    for p, g in zip(ps, (x[:1], plain[:1])):
+        AdamW([p], lr=0.1).step(grads=[g])
+    assert torch.equal(ps[0], ps[1]) and float(ps[0].detach()) != 0
+    neg = z.conj().imag[0]
+    for bad in (lambda: hip_ops.rms_norm_forward(plain, neg), lambda: hip_ops.rms_norm_backward(plain[:1], plain[:1], neg, one),
+                lambda: hip_ops.linear_w4(plain[:1], wq, scales, 20, x_scale=neg), lambda: AdamW([neg.detach().requires_grad_()])):
+        with pytest.raises(ValueError):
+            bad()
