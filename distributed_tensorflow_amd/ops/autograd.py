@@ -239,7 +239,9 @@ def avg_pool3x3_same(x: torch.Tensor) -> torch.Tensor:
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
     """``h = x + residual; y = h / sqrt(mean(h^2) + eps) * weight`` over the last dimension; ``y``, or ``(y, h)`` with a residual.
-    ``x`` and ``residual`` fp32 or bf16 of one shape and type, ``weight`` fp32; differentiable once in all three."""
+    ``x`` and ``residual`` fp32 or bf16 of one shape and type, ``weight`` fp32; differentiable once in all three (a second derivative
+    raises).  Forward and backward pass can be captured into a graph; as with any torch operation, no eager graph of the same leaves
+    may be alive then."""
     return native.ext().rms_norm(x, weight, residual, eps)
 
 
